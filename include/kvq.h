@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define KVQ_ABI_VERSION 6
+#define KVQ_ABI_VERSION 7
 
 /* Element types of queries, K/V rows, outputs, scales and biases. */
 #define KVQ_DTYPE_F16 0
@@ -240,6 +240,58 @@ int kvq_decode_attn_dense_masked(const kvq_rows* q, const kvq_rows* k, const kvq
                                  void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * A tree of drafted tokens (speculative decoding): the last L rows of a sequence's cache are its nodes, and
+ * query row l is node l. A node sees every key before the tree, its ancestors and itself; it sits at position
+ * (keys before the tree) + depth. bits: uint32 [B][L][ceil(L / 32)], bit j % 32 of word j / 32 of row l set if
+ * node j is l or an ancestor of l; depths: int32 [B][L], -1 for an absent node (padding in a batch of unequal
+ * trees), whose row of bits is zero and which no node sees. Batch strides in elements; 0: one tree for the
+ * whole batch. kvq_draft_tree writes both. No counterpart in the reference.
+ */
+#define KVQ_TREE_MAX_NODES 1024
+typedef struct kvq_tree {
+  const uint32_t* bits;
+  const int32_t* depths;
+  int64_t bits_stride_b, depths_stride_b;
+} kvq_tree;
+
+/*
+ * bits [B][L][ceil(L / 32)] and depths [B][L] (contiguous) of the trees whose nodes have the parents
+ * int32 [B][L] (batch stride parents_stride_b, 0 for B equal trees): -1 for a child of the last token before
+ * the tree, else the index of an earlier node. Any other value makes the node absent, and its descendants
+ * with it. positions (may be NULL; int32 [B][L]): starts[b] (or `start` where starts is NULL) + depth, of an
+ * absent node starts[b]. 1 <= L <= KVQ_TREE_MAX_NODES.
+ */
+int kvq_draft_tree(const int32_t* parents, int64_t parents_stride_b, int B, int L, uint32_t* bits, int32_t* depths,
+                   const int32_t* starts, int64_t start, int32_t* positions, void* stream);
+
+/*
+ * Attention of the L nodes of a tree over a quantized cache: kvq_decode_attn with the tree's visibility in
+ * place of a causal mask, for any L up to KVQ_TREE_MAX_NODES and the same head dims, groups and bits. An absent
+ * node's output row is 0.
+ *   seq_lens: NULL (S rows each) or device int32 [B], L <= seq_lens[b] <= S: the rows with the tree's.
+ *   window:   0 = none; else at least L: keys at positions > the node's position - window only.
+ * Calls of many rows run on the prefill kernels (head_dim 64, 96, 128 with output rows 16-byte aligned and, with two
+ * or more scale groups a row, 4-byte aligned scale and bias rows; 256), a bf16 cache's only with its range words
+ * (kvq_tree_on_prefill says where they are read). Hidden keys' values enter a product with zero: they have to
+ * be finite, as under the other masks. workspace: kvq_tree_workspace_size bytes, 256-byte aligned, zero-filled
+ * when it is allocated.
+ */
+int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
+                  const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size,
+                  int dtype, float scale, const kvq_tree* tree, int window, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+size_t kvq_tree_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window);
+
+/* 1 if kvq_tree_attn may take a kernel that reads a bf16 cache's range words at these sizes, else 0. */
+int kvq_tree_on_prefill(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window);
+
+/* The same over an unquantized cache (kvq_decode_attn_dense's arguments and head dims). */
+int kvq_tree_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
+                        const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
+                        const kvq_tree* tree, int window, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Attention for prefill chunks (any L): same contract as kvq_decode_attn, MFMA tiles with
  * K/V tiles dequantized into LDS. Replaces m5engine/attention.py:29-103 for L > 1.
  * Requirements: those of kvq_decode_attn; Hq a multiple of Hkv; at D = 64 or 128 the output rows
@@ -339,6 +391,12 @@ int kvq_paged_prefill_attn(const kvq_rows* q, const kvq_qtensor* k_pool, const k
                            int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int dtype,
                            float scale, int causal, int window,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* kvq_tree_attn over paged pools (seq_lens may not be NULL here; the kernels and results are the same). */
+int kvq_paged_tree_attn(const kvq_rows* q, const kvq_qtensor* k_pool, const kvq_qtensor* v_pool, int num_pages,
+                        const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
+                        int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int dtype, float scale,
+                        const kvq_tree* tree, int window, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Radix prefix cache over a page pool (host memory and host code only; no HIP calls).

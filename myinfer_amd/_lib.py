@@ -16,7 +16,7 @@ import torch  # noqa: F401  (binds the HIP runtime before libkvq.so is loaded)
 
 # The in-tree build, the only library this package loads.
 LIB_PATH = Path(__file__).resolve().parent / "libkvq.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -113,6 +113,21 @@ _DENSE_MASKED_ARGS = [
 ]
 
 
+TREE_MAX_NODES = 1024  # KVQ_TREE_MAX_NODES
+
+
+class Tree(ctypes.Structure):
+    """kvq_tree: the ancestor bits [B][L][ceil(L / 32)] and depths [B][L] of trees of drafted tokens."""
+
+    _fields_ = [("bits", c_void_p), ("depths", c_void_p), ("bits_stride_b", c_int64), ("depths_stride_b", c_int64)]
+
+
+_TREE_TAIL = [
+    c_float, POINTER(Tree), c_int,  # scale tree window
+    c_void_p, c_size_t, c_void_p,  # workspace bytes stream
+]
+
+
 class RadixInfo(ctypes.Structure):
     """kvq_radix_info: counters of a radix prefix cache."""
 
@@ -145,6 +160,14 @@ SIGNATURES = {
     ),
     "kvq_paged_decode_attn": (c_int, _PAGED_ATTN_ARGS),
     "kvq_paged_prefill_attn": (c_int, _PAGED_ATTN_ARGS),
+    "kvq_draft_tree": (
+        c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
+    ),
+    "kvq_tree_attn": (c_int, _ATTN_ARGS[:14] + _TREE_TAIL),
+    "kvq_tree_attn_dense": (c_int, _DENSE_ARGS[:12] + _TREE_TAIL),
+    "kvq_paged_tree_attn": (c_int, _PAGED_ATTN_ARGS[:17] + _TREE_TAIL),
+    "kvq_tree_workspace_size": (c_size_t, _WS_ARGS),
+    "kvq_tree_on_prefill": (c_int, [c_int] * 8),
     "kvq_radix_create": (c_void_p, [c_int, c_int]),
     "kvq_radix_destroy": (None, [c_void_p]),
     "kvq_radix_match_and_allocate": (

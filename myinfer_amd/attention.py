@@ -32,6 +32,8 @@ Masks (the reference accepts None, a string, or an array):
                         batch row (keys >= S_b masked), is recognised and runs as that structure;
                         any other boolean mask (per-head masks included) is read by the kernel
   additive float        all-zero runs unmasked; any other is added to the scores by the kernel
+  kernels.DraftTree     the queries are the nodes of a tree of drafted tokens: each sees the keys before the
+                        tree, its ancestors and itself
 General masks (kernels.masked_attention) run on the decode kernel, or on the prefill kernel where
 there are many rows and keys, broadcast as the reference broadcasts them on the same path; a row
 that sees no key returns 0.
@@ -171,6 +173,9 @@ def blocked_quantized_sdpa(queries: torch.Tensor, q_keys, q_values, scale: float
                                       window=window, seq_lens=seq_lens, group_size=group_size, bits=bits)
         if out is not None:
             return out
+    if isinstance(mask, kernels.DraftTree):
+        return kernels.attention(queries, tuple(q_keys), tuple(q_values), scale, window=window, seq_lens=seq_lens,
+                                 group_size=group_size, bits=bits, tree=mask)
     B, n_q_heads, L, D = queries.shape
     S = q_keys[0].shape[-2]
     try:
@@ -211,6 +216,8 @@ def fast_scaled_dot_product_attention(queries: torch.Tensor, keys: torch.Tensor,
     queries [B, Hq, L, D]; keys, values [B, Hkv, S, D] in the queries' dtype (float16/bfloat16,
     CUDA). Masks as for blocked_quantized_sdpa. Returns [B, Hq, L, D].
     """
+    if isinstance(mask, kernels.DraftTree):
+        return kernels.attention(queries, keys, values, scale, window=window, seq_lens=seq_lens, tree=mask)
     B, n_q_heads, L, D = queries.shape
     S = keys.shape[-2]
     try:

@@ -602,6 +602,138 @@ int kvq_decode_attn_dense_masked(const kvq_rows* q, const kvq_rows* k, const kvq
                     "decode_attn_dense_masked launch");
 }
 
+// ---- trees of drafted tokens
+
+int kvq_draft_tree(const int32_t* parents, int64_t parents_stride_b, int B, int L, uint32_t* bits, int32_t* depths,
+                   const int32_t* starts, int64_t start, int32_t* positions, void* stream) {
+  if (!parents || !bits || !depths) return fail(KVQ_ERR_INVALID, "parents, bits and depths must not be NULL");
+  if (B < 0 || L < 0) return fail(KVQ_ERR_INVALID, "negative shape (B=%d L=%d)", B, L);
+  if (L > KVQ_TREE_MAX_NODES || B > 65535)
+    return fail(KVQ_ERR_UNSUPPORTED, "a tree has at most %d nodes and a batch 65535 trees, got %d and %d", KVQ_TREE_MAX_NODES, L, B);
+  if (parents_stride_b < 0) return fail(KVQ_ERR_INVALID, "parents have a negative batch stride");
+  if (!aligned(parents, 4) || !aligned(bits, 4) || !aligned(depths, 4) || !aligned(starts, 4) || !aligned(positions, 4))
+    return fail(KVQ_ERR_INVALID, "parents, bits, depths, starts and positions must be 4-byte aligned");
+  if (B == 0 || L == 0) return ok();
+  return hip_status(kvq::launch_draft_tree(parents, parents_stride_b, B, L, bits, depths, starts, start, positions,
+                                           (hipStream_t)stream),
+                    "draft_tree launch");
+}
+
+static int check_tree(const kvq_tree* t, int L, int window) {
+  if (!t || !t->bits || !t->depths) return fail(KVQ_ERR_INVALID, "tree, tree->bits and tree->depths must not be NULL");
+  if (!aligned(t->bits, 4) || !aligned(t->depths, 4) || t->bits_stride_b < 0 || t->depths_stride_b < 0)
+    return fail(KVQ_ERR_INVALID, "tree bits and depths must be 4-byte aligned with non-negative batch strides");
+  if (L > KVQ_TREE_MAX_NODES) return fail(KVQ_ERR_UNSUPPORTED, "a tree has at most %d nodes, got L=%d", KVQ_TREE_MAX_NODES, L);
+  // an ancestor is then never outside the window of its descendants
+  if (window > 0 && window < L) return fail(KVQ_ERR_UNSUPPORTED, "a tree of %d nodes needs a window of at least as many keys, got %d", L, window);
+  return KVQ_OK;
+}
+
+// Whether a tree's rows are enough for the prefill kernels (the head_dim-256 one at 256 dims). The decode
+// kernel's time grows with its passes over the keys, a prefill kernel's with its row blocks and the split
+// merge: the line is the one that calls of several passes' rows have measured (kernels._auto_kernel).
+static bool tree_rows_on_prefill(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window, bool dense) {
+  const int64_t rows = (int64_t)(Hq / Hkv) * L, units = (int64_t)B * Hkv;
+  if (D == 96 && !dense) return rows > 64;
+  if (D != 64 && D != 128 && (D != 256 || dense)) return false;
+  const int per = 16 * group_size / D;
+  if (rows <= std::max(per, 8)) return false;
+  if (dense) return true;
+  const int64_t passes = (rows + per - 1) / per, keys = window > 0 ? std::min(S, window + L) : S;
+  const int64_t block = D == 256 ? 128 : 256, free_passes = D == 256 ? 3 : 4, limit = D == 256 ? 5 << 15 : 330000;
+  return !(rows < block && units * passes <= 512 && (passes - free_passes) * units * keys <= limit);
+}
+
+int kvq_tree_on_prefill(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || S <= 0 || D <= 0 || window < 0 || group_size <= 0 || Hq % Hkv) return 0;
+  return tree_rows_on_prefill(B, Hq, Hkv, L, D, S, group_size, window, false) ? 1 : 0;
+}
+
+// The kernel of a call is chosen by its rows; a call whose tensors the prefill kernels cannot take stays on the
+// decode kernel (unaligned output or scale rows, a bf16 cache without range words).
+static bool tree_on_prefill(const kvq_qtensor* k, const kvq_qtensor* v, const kvq_rows* out, int B, int Hq, int Hkv, int L,
+                            int D, int S, int group_size, int dtype, int window) {
+  if (!tree_rows_on_prefill(B, Hq, Hkv, L, D, S, group_size, window, false)) return false;
+  if (dtype == KVQ_DTYPE_BF16 && (!k->range_exp || !v->range_exp)) return false;
+  if (D == 256) return true;
+  if (!aligned(out->data, 16) || (out->stride_b | out->stride_h | out->stride_l) % 8) return false;
+  return D == 96 || check_prefill_sb(k, v, D, group_size) == KVQ_OK;
+}
+
+size_t kvq_tree_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window) {
+  size_t n = kvq_decode_workspace_size(B, Hq, Hkv, L, D, S, window);
+  if (n == 0 || Hq % Hkv) return 0;
+  if (D == 64 || D == 96 || D == 128) n = std::max(n, kvq::prefill_tree_bytes(B, Hq, Hkv, L, D, S, window));
+  return n;  // (the decode size covers the head_dim-256 kernel)
+}
+
+int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
+                  const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int dtype,
+                  float scale, const kvq_tree* tree, int window, void* workspace, size_t workspace_bytes, void* stream) {
+  if (check_head_dim(D, "tree attention")) return KVQ_ERR_UNSUPPORTED;
+  int rc = check_attn(q, k, v, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, window,
+                      kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window), workspace, workspace_bytes);
+  if (rc || (rc = check_tree(tree, L, window))) return rc;
+  hipError_t e;
+  if (!tree_on_prefill(k, v, out, B, Hq, Hkv, L, D, S, group_size, dtype, window)) {
+    e = kvq::launch_decode(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, 0, window, workspace,
+                           (hipStream_t)stream, nullptr, tree);
+  } else if (D == 256) {
+    e = kvq::launch_wide(q, k, v, seq_lens, out, B, Hq, Hkv, L, S, bits, group_size, dtype, scale, 0, window, workspace,
+                         (hipStream_t)stream, tree);
+  } else {
+    e = kvq::launch_prefill(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, 0, window, workspace,
+                            (hipStream_t)stream, tree);
+  }
+  return hip_status(e, "tree_attn launch");
+}
+
+int kvq_paged_tree_attn(const kvq_rows* q, const kvq_qtensor* k_pool, const kvq_qtensor* v_pool, int num_pages,
+                        const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
+                        int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int dtype, float scale,
+                        const kvq_tree* tree, int window, void* workspace, size_t workspace_bytes, void* stream) {
+  if (check_head_dim(D, "tree attention")) return KVQ_ERR_UNSUPPORTED;
+  int rc = check_paged_attn(q, k_pool, v_pool, num_pages, block_table, table_stride, out, B, Hq, Hkv, L, D, S, bits,
+                            group_size, dtype, scale, window, kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window),
+                            workspace, workspace_bytes);
+  if (rc || (rc = check_tree(tree, L, window))) return rc;
+  if (!seq_lens) return fail(KVQ_ERR_INVALID, "seq_lens is NULL");
+  hipError_t e;
+  if (!tree_on_prefill(k_pool, v_pool, out, B, Hq, Hkv, L, D, S, group_size, dtype, window)) {
+    e = kvq::launch_decode_paged(q, k_pool, v_pool, num_pages, block_table, table_stride, seq_lens, out, B, Hq, Hkv, L, D, S,
+                                 bits, group_size, dtype, scale, 0, window, workspace, (hipStream_t)stream, tree);
+  } else if (D == 256) {
+    e = kvq::launch_wide_paged(q, k_pool, v_pool, num_pages, block_table, table_stride, seq_lens, out, B, Hq, Hkv, L, S, bits,
+                               group_size, dtype, scale, 0, window, workspace, (hipStream_t)stream, tree);
+  } else {
+    e = kvq::launch_prefill_paged(q, k_pool, v_pool, num_pages, block_table, table_stride, seq_lens, out, B, Hq, Hkv, L, D, S,
+                                  bits, group_size, dtype, scale, 0, window, workspace, (hipStream_t)stream, tree);
+  }
+  return hip_status(e, "paged_tree_attn launch");
+}
+
+int kvq_tree_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
+                        const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
+                        const kvq_tree* tree, int window, void* workspace, size_t workspace_bytes, void* stream) {
+  if (check_head_dim(D, "unquantized tree attention")) return KVQ_ERR_UNSUPPORTED;
+  int rc = check_attn_dense(q, k, v, out, B, Hq, Hkv, L, D, S, dtype, scale, window,
+                            kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window), workspace, workspace_bytes);
+  if (rc || (rc = check_tree(tree, L, window))) return rc;
+  const bool rows16 = aligned(out->data, 16) && !((out->stride_b | out->stride_h | out->stride_l) % 8);
+  hipError_t e;
+  if (D > 128) {  // unquantized rows past 128 dims run through the head_dim-256 kernel
+    e = kvq::launch_wide_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,
+                               (hipStream_t)stream, nullptr, tree);
+  } else if (tree_rows_on_prefill(B, Hq, Hkv, L, D, S, 64, window, true) && (D == 64 || rows16)) {
+    e = kvq::launch_prefill_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,
+                                  (hipStream_t)stream, tree);
+  } else {
+    e = kvq::launch_decode_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,
+                                 (hipStream_t)stream, nullptr, tree);
+  }
+  return hip_status(e, "tree_attn_dense launch");
+}
+
 int kvq_prefill_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                            const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
                            int causal, int window, void* workspace, size_t workspace_bytes, void* stream) {

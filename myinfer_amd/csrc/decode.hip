@@ -101,16 +101,6 @@ size_t decode_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int w
   return decode_layout(pl, Dk).total;
 }
 
-// Whether kernel width D with scale group G serves narrower rows: head dims that run at width D
-// (decode_kernel_dim) and are multiples of G, i.e. 32 dims at width 64 (G 32), 96 at 128 (G 32) and
-// 192 at 256 (G 64); unquantized rows (G stands at 64) of any multiple of 8 at width 64 or 128.
-template <int D, int BITS, int G>
-constexpr bool narrow_rows() {
-  if constexpr (BITS == 16) return D <= 128;
-  const int lo = D == 64 ? 0 : D / 2;  // the widths below D end here
-  return (lo / G + 1) * G < D;
-}
-
 template <typename T, int D, int BITS, int NW, int NSLOT, bool PAGED = false, int G = 64>
 static hipError_t launch_decode_t(const DecParams& p, hipStream_t stream) {
   if (p.dv != D) {
@@ -222,7 +212,8 @@ static void set_mask(DecParams& p, const kvq_mask* mask) {
 
 hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                          const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,
-                         float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask) {
+                         float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask,
+                         const kvq_tree* tree) {
   const int Dk = decode_kernel_dim(D);
   const DecPlan pl = decode_plan(B, Hq, Hkv, L, Dk, S, window, bits, G);
   DecParams p = decode_params(q, seq_lens, out, Hq, Hkv, L, Dk, S, scale, causal, window, workspace, pl);
@@ -246,6 +237,10 @@ hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qten
   p.vsb_sb = v->sb_stride_b;
   p.vsb_sh = v->sb_stride_h;
   p.vsb_ss = v->sb_stride_s;
+  if (tree) {
+    p.tree = tree_params(tree, L);
+    return launch_decode_tree(p, dtype, Dk, bits, G, false, stream);
+  }
   if (!mask && D == Dk && multi_rows(p.nrows, pl.R)) return launch_decode_multi(p, dtype, Dk, bits, G, false, stream);
   return dispatch_quant(dtype, Dk, bits, G, [&](auto t, auto d, auto b, auto g) {
     return launch_decode_shape<decltype(t), decltype(d)::value, decltype(b)::value, decltype(g)::value>(p, pl, stream);
@@ -255,7 +250,7 @@ hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qten
 hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                                const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                                int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype, float scale,
-                               int causal, int window, void* workspace, hipStream_t stream) {
+                               int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const int Dk = decode_kernel_dim(D);
   const DecPlan pl = decode_plan(B, Hq, Hkv, L, Dk, S, window, bits, G);
   DecParams p = decode_params(q, seq_lens, out, Hq, Hkv, L, Dk, S, scale, causal, window, workspace, pl);
@@ -281,6 +276,10 @@ hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kv
   p.table = table;
   p.table_stride = table_stride;
   p.num_pages = num_pages;
+  if (tree) {
+    p.tree = tree_params(tree, L);
+    return launch_decode_tree(p, dtype, Dk, bits, G, true, stream);
+  }
   if (D == Dk && multi_rows(p.nrows, pl.R)) return launch_decode_multi(p, dtype, Dk, bits, G, true, stream);
   return dispatch_quant(dtype, Dk, bits, G, [&](auto t, auto d, auto b, auto g) {
     return launch_decode_t<decltype(t), decltype(d)::value, decltype(b)::value, 4, 2, true, decltype(g)::value>(p, stream);
@@ -289,7 +288,8 @@ hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kv
 
 hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                                const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
-                               int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask) {
+                               int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask,
+                               const kvq_tree* tree) {
   const int Dk = decode_kernel_dim(D);
   const DecPlan pl = decode_plan(B, Hq, Hkv, L, Dk, S, window, 16, 64);
   DecParams p = decode_params(q, seq_lens, out, Hq, Hkv, L, Dk, S, scale, causal, window, workspace, pl);
@@ -305,6 +305,10 @@ hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_r
   p.vc_ss = v->stride_l * 2;
   const bool bf = dtype == KVQ_DTYPE_BF16;
   if (Dk == 256) return hipErrorInvalidValue;  // unquantized rows past 128 dims run through the head_dim-256 kernel
+  if (tree) {
+    p.tree = tree_params(tree, L);
+    return launch_decode_tree(p, dtype, Dk, 16, 64, false, stream);
+  }
   if (Dk == 128) return bf ? launch_decode_shape<BF16, 128, 16>(p, pl, stream) : launch_decode_shape<F16, 128, 16>(p, pl, stream);
   return bf ? launch_decode_shape<BF16, 64, 16>(p, pl, stream) : launch_decode_shape<F16, 64, 16>(p, pl, stream);
 }

@@ -44,6 +44,7 @@
 #include "common.h"
 #include "launch.h"
 #include "merge.h"
+#include "tree.h"
 
 namespace kvq {
 
@@ -123,6 +124,8 @@ struct DecParams {
   int dv;
   // nsplit, rowblocks, Hkv and L as multiply-shift divisors (the workgroup and row numbering)
   Div31 d_nsplit, d_rowblocks, d_hkv, d_l;
+  // a tree of drafted tokens (TREE kernels): the last L rows of a sequence are its nodes
+  TreeParams tree;
 };
 
 // A general mask (kvq_mask) on the lane's 8 scores of a tile (keys k0 + 16 (s / 4) + 4 lg + s % 4 of
@@ -492,8 +495,10 @@ constexpr int dec_min_wgs() {
 // dims. The other instantiations carry no trace of either.
 // MULTI: for calls of several passes' rows, which the prefill kernels served before; they sum the
 // values with a rounding that is smaller than those kernels' (see the PV operand below).
+// TREE: query row l is node l of a tree of drafted tokens, which sees the keys before the tree and its
+// ancestors (tree.h); only the tiles that hold nodes look at the tree.
 template <typename T, int D, int BITS, int NW, int NSLOT, bool PAGED = false, int G = 64, bool MASKED = false,
-          bool NARROW = false, bool MULTI = false>
+          bool NARROW = false, bool MULTI = false, bool TREE = false>
 __global__ __launch_bounds__(NW * 64, (dec_min_wgs<D, BITS, NW, NSLOT, G>())) void decode_attn_kernel(DecParams p) {
   using C = DecCfg<D, BITS, G>;
   constexpr int R = C::R;
@@ -557,6 +562,8 @@ __global__ __launch_bounds__(NW * 64, (dec_min_wgs<D, BITS, NW, NSLOT, G>())) vo
   const int hq = kvh * p.rep + (row_ok ? rq : 0);
   const int lq = row_ok ? row - rq * p.L : 0;
   const bool in_group = (lg * (D / 4)) / G == g;
+  TreeRow node;
+  if constexpr (TREE) node.load(p.tree, b, lq, S_b - p.L);
   u4 qraw[C::KSTEPS];
   {
     const uint16_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh + (int64_t)lq * p.q_sl + lg * (D / 4);
@@ -656,11 +663,11 @@ __global__ __launch_bounds__(NW * 64, (dec_min_wgs<D, BITS, NW, NSLOT, G>())) vo
   for (int j = 0; j < NSLOT; ++j) issue(j, j);
   __builtin_amdgcn_sched_barrier(0);
 
-  const int qpos = S_b - p.L + lq;
+  const int qpos = S_b - p.L + (TREE ? node.depth : lq);
   const int lo_r = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
   const int hi_r = p.causal ? min(S_b, qpos + 1) : S_b;
   const int lo_all = p.window > 0 ? max(0, S_b - p.window) : 0;
-  const int hi_all = p.causal ? S_b - p.L + 1 : S_b;
+  const int hi_all = TREE || p.causal ? S_b - p.L + (TREE ? 0 : 1) : S_b;
 
   // ---- Q operand. Unquantized cache: the raw query slice itself (exact), the scale applied to the
   // fp32 scores. Quantized cache:
@@ -798,10 +805,15 @@ __global__ __launch_bounds__(NW * 64, (dec_min_wgs<D, BITS, NW, NSLOT, G>())) vo
     }
     const bool need_mask = MASKED || !(k0 >= lo_all && k0 + kTile <= hi_all);
     if (need_mask) {
+      uint32_t seen = ~0u;  // bit 16 (s / 4) + s % 4: key s of the lane
+      if constexpr (TREE) seen = node.keys(k0) >> (4 * lg);
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         const int t = k0 + 16 * (s >> 2) + 4 * lg + (s & 3);
         if (!(t >= lo_r && t < hi_r)) sc[s] = -INFINITY;
+        if constexpr (TREE) {
+          if (!((seen >> (16 * (s >> 2) + (s & 3))) & 1u)) sc[s] = -INFINITY;
+        }
       }
       if constexpr (MASKED) {
         if (row_ok) apply_mask(p, b, kvh, hq - kvh * p.rep, lq, k0, lg, lo_r, hi_r, sc);
@@ -947,6 +959,12 @@ __global__ __launch_bounds__(NW * 64, (dec_min_wgs<D, BITS, NW, NSLOT, G>())) vo
   float* const w_l = w_m + NW * R;     // [NW][R]
   float* const w_o = w_l + NW * R;     // [NW][R][D]
   float* const s_w = w_o + NW * R * D;  // [R][kMaxSplit]
+  if constexpr (TREE) {  // an absent node sees nothing
+    if (node.depth < 0) {
+      m_run = -INFINITY;
+      l_part = 0.0f;
+    }
+  }
   // ---- wave epilogue: sums over the 4 lane groups, then stage (m, l, o) in LDS
   l_part = add_xor32(add_xor16(l_part));
   ob_part = add_xor32(add_xor16(ob_part));
@@ -1181,6 +1199,19 @@ inline hipError_t dispatch_quant(int dtype, int D, int bits, int G, F&& f) {
   };
   return dtype == KVQ_DTYPE_BF16 ? by_d(BF16{}) : by_d(F16{});
 }
+
+// Whether kernel width D with scale group G serves narrower rows: head dims that run at width D
+// (decode_kernel_dim) and are multiples of G, i.e. 32 dims at width 64 (G 32), 96 at 128 (G 32) and
+// 192 at 256 (G 64); unquantized rows (G stands at 64) of any multiple of 8 at width 64 or 128.
+template <int D, int BITS, int G>
+constexpr bool narrow_rows() {
+  if constexpr (BITS == 16) return D <= 128;
+  const int lo = D == 64 ? 0 : D / 2;  // the widths below D end here
+  return (lo / G + 1) * G < D;
+}
+
+// decode_tree.hip: the TREE launches (p.tree set), any number of rows; bits 16: unquantized caches.
+hipError_t launch_decode_tree(const DecParams& p, int dtype, int D, int bits, int G, bool paged, hipStream_t stream);
 
 // decode_multi.hip: the MULTI launches, over contiguous caches and paged pools.
 hipError_t launch_decode_multi(const DecParams& p, int dtype, int D, int bits, int G, bool paged, hipStream_t stream);

@@ -25,29 +25,34 @@ hipError_t launch_rope(const kvq_rows* x, const kvq_rope_params* rope, int B, in
 // of the output are stored.
 int decode_kernel_dim(int D);
 size_t decode_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window, int bits, int G);
-// mask: a general mask (kvq_mask) or nullptr
+// mask: a general mask (kvq_mask) or nullptr; tree: a tree of drafted tokens (kvq_tree) or nullptr
 hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                          const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,
                          float scale, int causal, int window, void* workspace, hipStream_t stream,
-                         const kvq_mask* mask = nullptr);
+                         const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr);
 
 hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                                const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                                int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype, float scale,
-                               int causal, int window, void* workspace, hipStream_t stream);
+                               int causal, int window, void* workspace, hipStream_t stream,
+                               const kvq_tree* tree = nullptr);
 hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                                const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
                                int causal, int window, void* workspace, hipStream_t stream,
-                               const kvq_mask* mask = nullptr);
+                               const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr);
 
 size_t prefill_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
 hipError_t launch_prefill(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                           const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,
-                          float scale, int causal, int window, void* workspace, hipStream_t stream);
+                          float scale, int causal, int window, void* workspace, hipStream_t stream,
+                          const kvq_tree* tree = nullptr);
 hipError_t launch_prefill_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                                 const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                                 int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype, float scale,
-                                int causal, int window, void* workspace, hipStream_t stream);
+                                int causal, int window, void* workspace, hipStream_t stream,
+                                const kvq_tree* tree = nullptr);
+// The workspace of the launch_prefill* calls over a tree.
+size_t prefill_tree_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
 // Under a general mask: bits 16 over kd / vd (head_dim 64 or 128), else over k / v (64, 96 or 128);
 // workspace_bytes: what the call's shapes entitle it to, not the size of the caller's buffer.
 // prefill_masked_rows: whether the prefill kernel is the faster one for such a call; prefill_masked_bytes:
@@ -63,17 +68,22 @@ hipError_t launch_prefill_masked(const kvq_rows* q, const kvq_qtensor* k, const 
 size_t wide_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
 hipError_t launch_wide(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                        const kvq_rows* out, int B, int Hq, int Hkv, int L, int S, int bits, int G, int dtype,
-                       float scale, int causal, int window, void* workspace, hipStream_t stream);
+                       float scale, int causal, int window, void* workspace, hipStream_t stream,
+                       const kvq_tree* tree = nullptr);
 hipError_t launch_wide_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                              const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                              int B, int Hq, int Hkv, int L, int S, int bits, int G, int dtype, float scale, int causal,
-                             int window, void* workspace, hipStream_t stream);
+                             int window, void* workspace, hipStream_t stream, const kvq_tree* tree = nullptr);
 hipError_t launch_wide_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                              const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
                              int causal, int window, void* workspace, hipStream_t stream,
-                             const kvq_mask* mask = nullptr);
+                             const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr);
 hipError_t launch_prefill_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                                 const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype,
-                                float scale, int causal, int window, void* workspace, hipStream_t stream);
+                                float scale, int causal, int window, void* workspace, hipStream_t stream,
+                                const kvq_tree* tree = nullptr);
+// tree.hip: the bits and depths of a tree (kvq_draft_tree)
+hipError_t launch_draft_tree(const int32_t* parents, int64_t parents_sb, int B, int L, uint32_t* bits, int32_t* depths,
+                             const int32_t* starts, int64_t start, int32_t* positions, hipStream_t stream);
 
 }  // namespace kvq

@@ -130,39 +130,57 @@ static void dense_operands(PreParams& p, const kvq_rows* k, const kvq_rows* v) {
 
 hipError_t launch_prefill(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                           const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,
-                          float scale, int causal, int window, void* workspace, hipStream_t stream) {
+                          float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, causal);
   PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl,
-                               D == 96);
+                               D == 96 || tree);
   quant_operands(p, k, v);
+  if (tree) {
+    p.tree = tree_params(tree, L);
+    return launch_prefill_tree(p, dtype, D, bits, G, false, stream);
+  }
   return launch_prefill_quant<false>(p, dtype, D, bits, G, stream);
 }
 
 hipError_t launch_prefill_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                                 const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                                 int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype, float scale,
-                                int causal, int window, void* workspace, hipStream_t stream) {
+                                int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, causal);
   PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl,
-                               D == 96);
+                               D == 96 || tree);
   quant_operands(p, k, v);  // (batch strides are page strides)
   p.table = table;
   p.table_stride = table_stride;
   p.num_pages = num_pages;
+  if (tree) {
+    p.tree = tree_params(tree, L);
+    return launch_prefill_tree(p, dtype, D, bits, G, true, stream);
+  }
   return launch_prefill_quant<true>(p, dtype, D, bits, G, stream);
 }
 
 hipError_t launch_prefill_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                                 const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype,
-                                float scale, int causal, int window, void* workspace, hipStream_t stream) {
+                                float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, causal);
-  PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl, D == 64);
+  PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl, D == 64 || tree);
   dense_operands(p, k, v);
   p.out8 = ((uintptr_t)out->data % 16 || (out->stride_b | out->stride_h | out->stride_l) % 8) ? 1 : 0;
+  if (tree) {
+    p.tree = tree_params(tree, L);
+    return launch_prefill_tree(p, dtype, D, 16, 64, false, stream);
+  }
   const bool bf = dtype == KVQ_DTYPE_BF16;
   if (D == 64)
     return bf ? launch_prefill_t<BF16, 16, false, 64, 64>(p, stream) : launch_prefill_t<F16, 16, false, 64, 64>(p, stream);
   return bf ? launch_prefill_t<BF16, 16>(p, stream) : launch_prefill_t<F16, 16>(p, stream);
+}
+
+// ---- trees of drafted tokens (prefill_tree.hip): the plan of a call without a causal mask, fp32 partials
+size_t prefill_tree_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window) {
+  const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, 0);
+  return pl.nsplit > 1 ? prefill_layout(pl, D, true).total : kCounterBytes;
 }
 
 // ---- general masks (prefill_masked.hip)

@@ -44,6 +44,7 @@
 #include "launch.h"
 #include "merge.h"
 #include "prefill_plan.h"
+#include "tree.h"
 
 namespace kvq {
 
@@ -172,6 +173,8 @@ struct PreParams {
   const uint64_t* words;
   int nwords;  // words per bitmap
   int w_kv;    // 1: the bitmaps have a KV head axis
+  // a tree of drafted tokens (TREE kernels): the last L rows of a sequence are its nodes
+  TreeParams tree;
 };
 
 // The tiles of a row block that hold a visible key, under a general mask, and how the splits share
@@ -484,15 +487,19 @@ __device__ __forceinline__ void stage_v_raw(const uint8_t* raw, _Float16* vlds, 
 
 // Whether a split's partial rows are kept in fp32: for the calls that kernels with fp32 partials served before
 // this one (head_dim 96 and general masks the decode kernel, unquantized head_dim 64 the head_dim-256
-// kernel's form of that width). The others pack them to fp16, which their workspaces are sized for.
-template <int BITS, int D, int MASKED>
-constexpr bool kF32Partials = MASKED != 0 || D == 96 || (BITS == 16 && D == 64);
+// kernel's form of that width), and for trees of drafted tokens. The others pack them to fp16, which their
+// workspaces are sized for.
+template <int BITS, int D, int MASKED, bool TREE = false>
+constexpr bool kF32Partials = MASKED != 0 || TREE || D == 96 || (BITS == 16 && D == 64);
 
 // MASKED: 0, or under a general mask: 1 boolean, 2 additive. The tile loop then walks the list of tiles
 // with a visible key, and reads the mask beside those that are not visible as a whole.
-template <typename T, int BITS, bool PAGED = false, int G = 64, int D = 128, int MASKED = 0>
+// TREE: query row l is node l of a tree of drafted tokens, which sees the keys before the tree and its
+// ancestors (tree.h); only the blocks of keys that hold nodes look at the tree.
+template <typename T, int BITS, bool PAGED = false, int G = 64, int D = 128, int MASKED = 0, bool TREE = false>
 __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) {
   static_assert(!(PAGED && MASKED), "general masks: contiguous caches");
+  static_assert(!(TREE && MASKED), "a tree or a general mask");
   using RC = RawCfg<BITS, G, D>;
   constexpr bool DENSE = RC::DENSE;  // unquantized cache: K operands are read from the raw ring
   constexpr int KS = kKS<D>;
@@ -527,14 +534,14 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
   if constexpr (MASKED) {
     ms = split_masked(p, b, kvh, rb);
   } else {
-    ks = split_keys(p, S_b, fr0, frl);
+    ks = split_keys(p, S_b, TREE ? 0 : fr0, frl);  // (any node may be as shallow as the first)
   }
   const int nsplit = MASKED ? ms.nsplit : ks.nsplit;
   if (split >= nsplit) return;
   const int pos_min = S_b - p.L + fr0 / p.rep, pos_max = S_b - p.L + frl / p.rep;
   // keys every row of the workgroup sees: tiles inside need no mask
-  const int hi_all = p.causal ? min(S_b, pos_min + 1) : S_b;
-  const int lo_all = p.window > 0 ? max(0, pos_max - p.window + 1) : 0;
+  const int hi_all = TREE ? S_b - p.L : p.causal ? min(S_b, pos_min + 1) : S_b;
+  const int lo_all = p.window > 0 ? max(0, (TREE ? S_b - 1 : pos_max) - p.window + 1) : 0;
   int k_begin = 0, ntile;  // tile starts stay 64-aligned
   if constexpr (MASKED) {
     ntile = __builtin_amdgcn_readfirstlane(max(min(ms.chunk, ms.n - split * ms.chunk), 0));
@@ -583,7 +590,9 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
   const bool row_ok = fr < p.nrows;
   const int lq = row_ok ? fr / p.rep : 0;
   const int head = kvh * p.rep + (row_ok ? fr % p.rep : 0);
-  const int pos = S_b - p.L + lq;
+  TreeRow node;
+  if constexpr (TREE) node.load(p.tree, b, lq, S_b - p.L);
+  const int pos = S_b - p.L + (TREE ? node.depth : lq);
   const int lo_r = p.window > 0 ? max(0, pos - p.window + 1) : 0;
   const int hi_r = p.causal ? min(S_b, pos + 1) : S_b;
 
@@ -766,6 +775,16 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
       }
     }
   };
+  // a tree's 32-key block from k: this lane's keys k + 8 (i / 4) + 4 hh + i % 4
+  auto tree_mask = [&](f16v& acc, int k) {
+    const uint32_t seen = node.keys(k) >> (4 * hh);
+    const int lo = lo_r - k - 4 * hh;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = 8 * (i >> 2) + (i & 3);
+      if (c < lo || !((seen >> c) & 1u)) acc[i] = -INFINITY;
+    }
+  };
   // MFMA operand type: bf16 for an unquantized bf16 cache, else fp16
   using OT = typename std::conditional<DENSE && T::id == KVQ_DTYPE_BF16, BF16, F16>::type;
 
@@ -788,6 +807,13 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
         return;
       }
       const bool need_mask = !(k0 >= lo_all && k0 + kPT <= hi_all);
+      if constexpr (TREE) {
+        if (__builtin_expect(need_mask, 0)) {
+          tree_mask(acc[0], k0);
+          tree_mask(acc[1], k0 + 32);
+        }
+        return;
+      }
       if (__builtin_expect(need_mask, 0)) {
         const int lo = lo_r - k0 - 4 * hh, hi = hi_r - k0 - 4 * hh;
         if (lo <= 0) {  // no key of the tile is below the lane's window
@@ -939,6 +965,10 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
         return;
       }
       if (__builtin_expect(!(k >= lo_all && k + 32 <= hi_all), 0)) {
+        if constexpr (TREE) {
+          tree_mask(acc, k);
+          return;
+        }
         const int lo = lo_r - k - 4 * hh, hi = hi_r - k - 4 * hh;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1115,6 +1145,15 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
     }
   }
 
+  if constexpr (TREE) {  // an absent node sees nothing
+    if (node.depth < 0) {
+      m_run = -INFINITY;
+      l_run = 0.0f;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) oacc[db] = f16v{};
+    }
+  }
+
   // ---- epilogue: this lane holds O^T[d][row] for d = 32db + 8(i/4) + 4hh + i%4
   float l_tot = add_xor32(l_run);
   if (nsplit > 1) {
@@ -1131,7 +1170,7 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
     //    Record of row r at byte 16 (s * kPRows + r) of the unit's record block.
     //  * With fp32 partials (kF32Partials) a row is o itself in the cache's units, word u (0 .. 2 QW - 1) value
     //    group u, and its record (m, l), 8 bytes: the merge scales row s by w_s.
-    constexpr bool F32P = kF32Partials<BITS, D, MASKED>;
+    constexpr bool F32P = kF32Partials<BITS, D, MASKED, TREE>;
     constexpr int NW = F32P ? 2 * QW : QW;       // 16-byte words of a lane's row
     constexpr uint32_t split_o = kPW * NW * 1024;
     const __amdgpu_buffer_rsrc_t ro =
@@ -1305,7 +1344,7 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
 // 16-byte word u of the packed rows of one wave (32 rows) of a row block; its 8 waves take the splits
 // in turn, four in flight each, and wave 0 sums the eight partial merges. Row blocks that were not
 // split have been written already. F32P: the partials are fp32 (kF32Partials), a word 4 values of a row rather than 8.
-template <typename T, int D, bool F32P, bool MASKED = false>
+template <typename T, int D, bool F32P, bool MASKED = false, bool TREE = false>
 __global__ __launch_bounds__(kPW * 64) void prefill_combine_kernel(PreParams p) {
   constexpr int QW = F32P ? D / 8 : D / 16;  // words per row
   constexpr int NV = F32P ? 4 : 8;           // values per word
@@ -1326,7 +1365,7 @@ __global__ __launch_bounds__(kPW * 64) void prefill_combine_kernel(PreParams p) 
   if constexpr (MASKED) {
     ks.nsplit = split_masked(p, b, kvh, rb).nsplit;
   } else {
-    ks.nsplit = split_keys(p, S_b, fr0, frl).nsplit;
+    ks.nsplit = split_keys(p, S_b, TREE ? 0 : fr0, frl).nsplit;
   }
   if (ks.nsplit == 1 || fr0 + 32 * w >= p.nrows) return;
   const uint8_t* po = (const uint8_t*)p.part_o + (int64_t)unit * p.nsplit * split_o + (w * QW + u) * 1024 + 16 * lane;
@@ -1406,5 +1445,8 @@ __global__ __launch_bounds__(kPW * 64) void prefill_combine_kernel(PreParams p) 
 
 // prefill_masked.hip: the MASKED launches and the kernel that classes the mask's tiles.
 hipError_t launch_prefill_masked_t(const PreParams& p, int B, int dtype, int D, int bits, int G, hipStream_t stream);
+
+// prefill_tree.hip: the TREE launches (p.tree set); bits 16: unquantized caches.
+hipError_t launch_prefill_tree(const PreParams& p, int dtype, int D, int bits, int G, bool paged, hipStream_t stream);
 
 }  // namespace kvq

@@ -40,6 +40,7 @@
 #include "dma.h"
 #include "launch.h"
 #include "merge.h"
+#include "tree.h"
 
 namespace kvq {
 
@@ -120,6 +121,8 @@ struct WideParams {
   // the head dimension of the rows (NARROW kernels: a multiple of 8 below D, the unquantized rows
   // past 128 dims): their queries' dims from dv on are zero and only dv dims are stored
   int dv;
+  // a tree of drafted tokens (TREE kernels): the last L rows of a sequence are its nodes
+  TreeParams tree;
 };
 
 // A general mask (kvq_mask) on the lane's 16 scores of a tile (keys k0 + 8 (i / 4) + 4 h + i % 4 of
@@ -290,8 +293,9 @@ __device__ __forceinline__ void wide_stage_v(const uint8_t* raw, uint8_t* vop, i
 }
 
 // MASKED: compiled with a general mask (kvq_mask) read beside every tile; the other instantiations
-// carry no trace of it.
-template <typename T, int D, int BITS, int G, bool PAGED = false, bool MASKED = false, bool NARROW = false>
+// carry no trace of it. TREE: query row l is node l of a tree of drafted tokens, which sees the keys
+// before the tree and its ancestors (tree.h); only the tiles that hold nodes look at the tree.
+template <typename T, int D, int BITS, int G, bool PAGED = false, bool MASKED = false, bool NARROW = false, bool TREE = false>
 __global__ __launch_bounds__(kWW * 64, 1) void wide_attn_kernel(WideParams p) {
   using C = WideCfg<D, BITS, G>;
   static_assert(!NARROW || C::DENSE, "narrow rows: unquantized caches");
@@ -319,7 +323,8 @@ __global__ __launch_bounds__(kWW * 64, 1) void wide_attn_kernel(WideParams p) {
   const bool one_head = r0 / p.L == r1 / p.L;
   const int lq_min = one_head ? r0 % p.L : 0, lq_max = one_head ? r1 % p.L : p.L - 1;
   const int key_hi = p.causal ? min(S_b, max(0, S_b - p.L + lq_max + 1)) : S_b;
-  const int key_lo = p.window > 0 ? min(key_hi, max(0, S_b - p.L + lq_min - p.window + 1)) : 0;
+  // (any node of a tree may be as shallow as the first)
+  const int key_lo = p.window > 0 ? min(key_hi, max(0, S_b - p.L + (TREE ? 0 : lq_min) - p.window + 1)) : 0;
   const int t_lo = key_lo / kWT, t_hi = (key_hi + kWT - 1) / kWT;
   const int cps = (t_hi - t_lo + p.nsplit - 1) / p.nsplit;
   const int t_begin = min(t_hi, t_lo + split * cps), t_end = min(t_hi, t_begin + cps);
@@ -413,12 +418,14 @@ __global__ __launch_bounds__(kWW * 64, 1) void wide_attn_kernel(WideParams p) {
   const bool row_ok = row < p.nrows;
   const int hq = kvh * p.rep + (row_ok ? row / p.L : 0);
   const int lq = row_ok ? row % p.L : 0;
-  const int qpos = S_b - p.L + lq;
+  TreeRow node;
+  if constexpr (TREE) node.load(p.tree, b, lq, S_b - p.L);
+  const int qpos = S_b - p.L + (TREE ? node.depth : lq);
   const int lo_r = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
   const int hi_r = p.causal ? min(S_b, qpos + 1) : S_b;
   // keys every row of the block sees: tiles inside need no mask
-  const int lo_all = p.window > 0 ? max(0, S_b - p.L + lq_max - p.window + 1) : 0;
-  const int hi_all = p.causal ? S_b - p.L + lq_min + 1 : S_b;
+  const int lo_all = p.window > 0 ? max(0, S_b - p.L + (TREE ? p.L - 1 : lq_max) - p.window + 1) : 0;
+  const int hi_all = TREE ? S_b - p.L : p.causal ? S_b - p.L + lq_min + 1 : S_b;
 
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -497,10 +504,15 @@ __global__ __launch_bounds__(kWW * 64, 1) void wide_attn_kernel(WideParams p) {
     }
     // value i of the lane is key k0 + 8 (i / 4) + 4 h + i % 4 of query row n
     if (MASKED || !(k0 >= lo_all && k0 + kWT <= hi_all)) {
+      uint32_t seen = ~0u;  // bit 8 (i / 4) + i % 4: key i of the lane
+      if constexpr (TREE) seen = node.keys(k0) >> (4 * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int k = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
         if (k < lo_r || k >= hi_r) s[i] = -INFINITY;
+        if constexpr (TREE) {
+          if (!((seen >> (8 * (i >> 2) + (i & 3))) & 1u)) s[i] = -INFINITY;
+        }
       }
       if constexpr (MASKED) {
         float sv[16];
@@ -601,6 +613,15 @@ __global__ __launch_bounds__(kWW * 64, 1) void wide_attn_kernel(WideParams p) {
     }
   }
 
+  if constexpr (TREE) {  // an absent node sees nothing
+    if (node.depth < 0) {
+      m_run = -INFINITY;
+      l_tot = 0.0f;
+#pragma unroll
+      for (int db = 0; db < C::NDB; ++db) oacc[db] = f16v{};
+    }
+  }
+
   // ---- epilogue: lane (n, h) holds O^T rows 32 db + 8 i + 4 h + j (j = 0..3) of query row n
   if (!row_ok) return;
   if (p.nsplit == 1) {
@@ -662,7 +683,16 @@ size_t wide_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int win
 
 template <typename T, int D, int BITS, int G, bool PAGED = false>
 static hipError_t launch_wide_t(const WideParams& p, hipStream_t stream) {
-  if (p.dv != D) {
+  const dim3 grid(p.nunits * p.nsplit), block(kWW * 64);
+  if (p.tree.bits) {
+    if (p.dv == D) {
+      hipLaunchKernelGGL((wide_attn_kernel<T, D, BITS, G, PAGED, false, false, true>), grid, block, 0, stream, p);
+    } else if constexpr (BITS == 16 && !PAGED) {
+      hipLaunchKernelGGL((wide_attn_kernel<T, D, BITS, G, PAGED, false, true, true>), grid, block, 0, stream, p);
+    } else {
+      return hipErrorInvalidValue;
+    }
+  } else if (p.dv != D) {
     // unquantized rows narrower than 256 dims (decode_kernel_dim), plain or masked
     if constexpr (D == 256 && BITS == 16 && !PAGED) {
       if (p.mask_kind != 0) {
@@ -776,8 +806,9 @@ static hipError_t launch_wide_quant(const WideParams& p, int bits, int G, int dt
 
 hipError_t launch_wide(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                        const kvq_rows* out, int B, int Hq, int Hkv, int L, int S, int bits, int G, int dtype,
-                       float scale, int causal, int window, void* workspace, hipStream_t stream) {
+                       float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   WideParams p = wide_params(q, seq_lens, out, B, Hq, Hkv, L, S, scale, causal, window, workspace);
+  if (tree) p.tree = tree_params(tree, L);
   wide_quant_params(p, k, v);
   return launch_wide_quant<false>(p, bits, G, dtype, stream);
 }
@@ -786,8 +817,9 @@ hipError_t launch_wide(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtenso
 hipError_t launch_wide_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                              const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                              int B, int Hq, int Hkv, int L, int S, int bits, int G, int dtype, float scale, int causal,
-                             int window, void* workspace, hipStream_t stream) {
+                             int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   WideParams p = wide_params(q, seq_lens, out, B, Hq, Hkv, L, S, scale, causal, window, workspace);
+  if (tree) p.tree = tree_params(tree, L);
   wide_quant_params(p, k, v);
   p.table = table;
   p.table_stride = table_stride;
@@ -797,8 +829,10 @@ hipError_t launch_wide_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_
 
 hipError_t launch_wide_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                              const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
-                             int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask) {
+                             int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask,
+                             const kvq_tree* tree) {
   WideParams p = wide_params(q, seq_lens, out, B, Hq, Hkv, L, S, scale, causal, window, workspace);
+  if (tree) p.tree = tree_params(tree, L);
   if (mask) {
     p.mask = mask->data;
     p.mask_kind = mask->kind;

@@ -7,6 +7,7 @@ zero-filled torch allocation cached per (device, stream); the library itself all
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import weakref
@@ -45,6 +46,13 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
         if t.device != dev:
             raise ValueError(f"all tensors must be on {dev}; got {t.device}")
     return dev
+
+
+def _on_device(dev: torch.device):
+    """A context in which `dev` is the current device (launches go to streams of the current one)."""
+    if dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 def _check_triple(tr: Sequence[torch.Tensor], name: str) -> None:
@@ -359,6 +367,72 @@ def _auto_kernel(rep_rows: int, D: int, group_size: int, *, dense: bool, units: 
     return "prefill"
 
 
+class DraftTree:
+    """The tokens drafted after a sequence's last one, as a tree (speculative decoding): what a node sees in
+    attention and where it sits.
+
+    ``parents``: int32 [B, L] (or [L], one tree for the whole batch) on the GPU, the parent of each node: -1 for
+    a child of the last token before the tree, else the index of an earlier node. Any other value makes
+    the node absent, and its descendants with it: padding, where the trees of a batch are unequal. Node l is row
+    S_b - L + l of the cache; it sees every key before the tree, its ancestors and itself, and an absent node
+    nothing (its output row is 0).
+
+    Built by one launch on the current stream; the layers of a step share it, as the mask of their attention
+    calls (``attention.scaled_dot_product_attention(..., mask=tree)``, ``attention(..., tree=tree)``).
+
+    ``depths`` [B, L] int32 are the nodes' depths (-1: absent). ``positions`` [1, B, L] int32, where ``starts`` (int32
+    [B] on the GPU, or one int: the position of a depth-0 node) was given, are the nodes' positions for
+    ``rope_axes``. ``refresh()`` launches again over the same buffers, after ``parents`` or ``starts`` were
+    refilled in place (and into a graph)."""
+
+    def __init__(self, parents: torch.Tensor, starts=None):
+        dev = _require_cuda(parents)
+        if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or parents.shape[-1] < 1:
+            raise ValueError(f"parents must be int32 [B, L] or [L] with L >= 1, got {parents.dtype} {tuple(parents.shape)}")
+        L = parents.shape[-1]
+        if L > _lib.TREE_MAX_NODES:
+            raise NotImplementedError(f"a tree has at most {_lib.TREE_MAX_NODES} nodes, got {L}")
+        if parents.stride(-1) != 1 and L > 1:
+            raise ValueError("the nodes of parents must be contiguous")
+        self.parents = parents
+        self.shared = parents.dim() == 1  # one tree for any batch
+        self.B, self.L = (1 if self.shared else parents.shape[0]), L
+        self._starts, self._start = None, 0
+        if torch.is_tensor(starts):
+            if starts.dtype != torch.int32 or starts.device != dev or tuple(starts.shape) != (self.B,) or \
+                    not starts.is_contiguous():
+                raise ValueError(f"starts must be an int or a contiguous int32 tensor of {self.B} entries on {dev}")
+            self._starts = starts
+        elif starts is not None:
+            self._start = int(starts)
+            if not -2 ** 31 <= self._start < 2 ** 31 - L:
+                raise ValueError(f"start {self._start} leaves the int32 positions")
+        words = (L + 31) // 32
+        n = self.B * L
+        buf = torch.empty(n * (words + (2 if starts is not None else 1)), dtype=torch.int32, device=dev)
+        self.bits = buf[: n * words].view(self.B, L, words)
+        self.depths = buf[n * words: n * (words + 1)].view(self.B, L)
+        self.positions = None if starts is None else buf[n * (words + 1):].view(1, self.B, L)
+        self.desc = _lib.Tree(self.bits.data_ptr(), self.depths.data_ptr(), 0 if self.shared else L * words,
+                              0 if self.shared else L)
+        self.device = dev
+        self.refresh()
+
+    def refresh(self) -> None:
+        with _on_device(self.device):
+            rc = _lib.lib().kvq_draft_tree(
+                self.parents.data_ptr(), 0 if self.shared else self.parents.stride(0), self.B, self.L, self.bits.data_ptr(),
+                self.depths.data_ptr(), None if self._starts is None else self._starts.data_ptr(), self._start,
+                None if self.positions is None else self.positions.data_ptr(), _lib.stream_ptr(self.device))
+        _lib.check(rc, "kvq_draft_tree")
+
+    def check(self, B: int, L: int, device) -> None:
+        """Raise unless queries [B, *, L, *] on `device` can be this tree's nodes."""
+        if self.L != L or (not self.shared and self.B != B) or self.device != device:
+            raise ValueError(f"the tree has {self.L} nodes for a batch of {'any' if self.shared else self.B} on "
+                             f"{self.device}; the queries are {L} rows for {B} on {device}")
+
+
 class AttentionCall:
     """A validated attention launch with its C-ABI arguments built once.
 
@@ -417,7 +491,8 @@ def _copy_for_one_shot(t: torch.Tensor, name: str, one_shot: bool) -> torch.Tens
 def prepare_attention(queries: torch.Tensor, keys, values, scale: float, *, causal: bool = False,
                       window: int = 0, seq_lens: Optional[torch.Tensor] = None, group_size: int = 64,
                       bits: int = 8, out: Optional[torch.Tensor] = None, kernel: str = "auto",
-                      workspace: Optional[torch.Tensor] = None, _one_shot: bool = False) -> AttentionCall:
+                      workspace: Optional[torch.Tensor] = None, tree: Optional[DraftTree] = None,
+                      _one_shot: bool = False) -> AttentionCall:
     """Validate one attention launch and return it as an ``AttentionCall`` (see ``attention``).
 
     The queries and unquantized keys/values must be readable in place (unit stride along D, 16-byte
@@ -467,6 +542,10 @@ def prepare_attention(queries: torch.Tensor, keys, values, scale: float, *, caus
             raise ValueError("seq_lens must be an int32 tensor of B entries on the queries' device")
         sl_ptr = seq_lens.data_ptr()
     rep = Hq // Hkv
+    if tree is not None:
+        return _prepare_tree(queries, keys, values, scale, tree, out, dense=dense, window=window, seq_lens=seq_lens,
+                             group_size=group_size, bits=bits, causal=causal, kernel=kernel, workspace=workspace,
+                             one_shot=_one_shot)
     if kernel == "auto":
         kernel = _auto_kernel(rep * L, D, 64 if dense else group_size, dense=dense, units=B * Hkv,
                               keys=min(S, window + L) if window else S)
@@ -509,6 +588,89 @@ def prepare_attention(queries: torch.Tensor, keys, values, scale: float, *, caus
     return AttentionCall(fn, args, keep, kernel, out, symbol)
 
 
+_COUNTER_BYTES = 1 << 18  # the arrival counters at the start of a workspace, zero before its first call
+
+
+def _tree_workspace(dev: torch.device, stream: int, nbytes: int, workspace: Optional[torch.Tensor]) -> torch.Tensor:
+    """The caller's workspace after its checks, or the stream's. A call that is captured into a graph without one
+    gets its own from the graph's memory (its counters cleared by a fill in every replay): graphs that were
+    captured on one stream may be replayed at once on others."""
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous() or \
+                workspace.numel() * workspace.element_size() < nbytes:
+            raise ValueError(f"workspace must hold at least {nbytes} contiguous bytes on {dev}")
+        return workspace
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(max(nbytes, _COUNTER_BYTES), dtype=torch.uint8, device=dev)
+        ws[:_COUNTER_BYTES].zero_()
+        return ws
+    return _workspace(dev, stream, nbytes)
+
+
+class _DeviceCall(AttentionCall):
+    """An AttentionCall whose launch makes its tensors' device the current one."""
+
+    def __init__(self, dev: torch.device, *args):
+        super().__init__(*args)
+        self._dev = dev
+
+    def __call__(self) -> torch.Tensor:
+        with _on_device(self._dev):
+            return super().__call__()
+
+
+def _check_tree_call(tree: DraftTree, B: int, L: int, S: int, window: int, causal: bool, kernel: str, device) -> None:
+    tree.check(B, L, device)
+    if causal or kernel != "auto":
+        raise ValueError("a tree says what its nodes see and which kernel serves them: no causal= or kernel= with tree=")
+    if S < L:
+        raise ValueError(f"the tree's {L} nodes are the last rows of the cache, which has {S}")
+    if window < 0:
+        raise ValueError(f"window must be >= 0, got {window}")
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_sizes(*sizes: int) -> Tuple[int, int]:
+    """(workspace bytes, whether a bf16 cache's range words are read) of a tree call, which follow from its sizes."""
+    B, Hq, Hkv, L, D, S, group_size, window = sizes
+    lib = _lib.lib()
+    return (lib.kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window),
+            lib.kvq_tree_on_prefill(B, Hq, Hkv, L, D, S, group_size, window))
+
+
+def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq_lens, group_size, bits, causal, kernel,
+                  workspace, one_shot) -> AttentionCall:
+    """prepare_attention's call over a tree (its tensors have been checked there)."""
+    B, Hq, L, D = queries.shape
+    dev = queries.device
+    Hkv, S = keys.shape[1:3] if dense else keys[0].shape[1:3]
+    _check_tree_call(tree, B, L, S, window, causal, kernel, dev)
+    nbytes, prefill = _tree_sizes(B, Hq, Hkv, L, D, S, 64 if dense else group_size, int(window))
+    if nbytes == 0:
+        raise NotImplementedError(f"tree attention does not support B={B} Hq={Hq} Hkv={Hkv} L={L} D={D} S={S}")
+    stream = _lib.stream_ptr(dev)
+    with _on_device(dev):
+        ws = _tree_workspace(dev, stream, nbytes, workspace)
+    qr, orr = _lib.rows(queries), _lib.rows(out)
+    kw = vw = None
+    if dense:
+        symbol, kq, vq, form = "kvq_tree_attn_dense", _lib.rows(keys), _lib.rows(values), ()
+    else:
+        # a bf16 cache's range words, as prepare_attention has them
+        if prefill and queries.dtype == torch.bfloat16:
+            kw, vw = range_word(keys[0]), range_word(values[0])
+            if one_shot:
+                kw = range_exponent(keys, bits) if kw is None else kw
+                vw = range_exponent(values, bits) if vw is None else vw
+        symbol, form = "kvq_tree_attn", (int(bits), int(group_size))
+        kq, vq = _lib.qtensor(*keys, range_exp=kw), _lib.qtensor(*values, range_exp=vw)
+    args = (ctypes.byref(qr), ctypes.byref(kq), ctypes.byref(vq), None if seq_lens is None else seq_lens.data_ptr(),
+            ctypes.byref(orr), B, Hq, Hkv, L, D, S, *form, _lib.dtype_code(queries.dtype), float(scale),
+            ctypes.byref(tree.desc), int(window), ws.data_ptr(), ws.numel() * ws.element_size(), stream)
+    keep = (queries, keys, values, seq_lens, ws, qr, orr, kq, vq, tree, kw, vw)
+    return _DeviceCall(dev, getattr(_lib.lib(), symbol), args, keep, "tree", out, symbol)
+
+
 def layer_attention(queries: torch.Tensor, keys, values, scale: float, *, causal: bool, window: int = 0,
                     seq_lens: Optional[torch.Tensor] = None, group_size: int = 64,
                     bits: int = 8) -> Optional[torch.Tensor]:
@@ -547,14 +709,18 @@ def layer_attention(queries: torch.Tensor, keys, values, scale: float, *, causal
 
 def attention(queries: torch.Tensor, keys, values, scale: float, *, causal: bool = False,
               window: int = 0, seq_lens: Optional[torch.Tensor] = None, group_size: int = 64, bits: int = 8,
-              out: Optional[torch.Tensor] = None, kernel: str = "auto") -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, kernel: str = "auto",
+              tree: Optional[DraftTree] = None) -> torch.Tensor:
     """softmax(scale * q K^T + mask) V. queries [B, Hq, L, D]; keys/values either quantized triples
     (codes [B, Hkv, S, D*bits/32], scales/biases [B, Hkv, S, D/G]) or unquantized tensors
     [B, Hkv, S, D] in the queries' dtype; returns [B, Hq, L, D] (or fills `out`). kernel: "decode",
     "prefill" or "auto" (decode while a KV head's query rows fit max(16*G/D, 8) columns, and past
-    that where its passes over the keys cost less than the prefill kernel's row blocks)."""
+    that where its passes over the keys cost less than the prefill kernel's row blocks).
+
+    With `tree` the queries are the nodes of a DraftTree, whose keys are each sequence's last L rows (of
+    seq_lens[b] >= L, or of S); a window must then be at least L."""
     return prepare_attention(queries, keys, values, scale, causal=causal, window=window, seq_lens=seq_lens,
-                             group_size=group_size, bits=bits, out=out, kernel=kernel, _one_shot=True)()
+                             group_size=group_size, bits=bits, out=out, kernel=kernel, tree=tree, _one_shot=True)()
 
 
 # ---- general masks (kvq_mask): boolean masks with no causal / window / padding structure, per-head
@@ -729,10 +895,12 @@ def paged_quantize_append(k: torch.Tensor, k_pool: Triple, v: Optional[torch.Ten
 def paged_attention(queries: torch.Tensor, k_pool: Triple, v_pool: Triple, block_tables: torch.Tensor,
                     seq_lens: torch.Tensor, scale: float, *, causal: bool = False, window: int = 0,
                     group_size: int = 64, bits: int = 8, max_len: Optional[int] = None,
-                    out: Optional[torch.Tensor] = None, kernel: str = "auto") -> torch.Tensor:
+                    out: Optional[torch.Tensor] = None, kernel: str = "auto", tree: Optional[DraftTree] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale * q K^T + mask) V over paged pools: sequence b holds seq_lens[b] rows in the
-    pages block_tables[b]; queries [B, Hq, L, D] sit at its last L positions. max_len bounds
-    seq_lens (default: the table's capacity) and sizes the split plan."""
+    pages block_tables[b]; queries [B, Hq, L, D] sit at its last L positions (or are the nodes of `tree`,
+    which those rows hold; `workspace` is then the caller's, if given). max_len bounds seq_lens (default: the
+    table's capacity) and sizes the split plan."""
     _check_triple(k_pool, "k_pool")
     _check_triple(v_pool, "v_pool")
     dev = _require_cuda(queries, *k_pool, *v_pool)
@@ -758,6 +926,26 @@ def paged_attention(queries: torch.Tensor, k_pool: Triple, v_pool: Triple, block
     if not _rows_ok(queries):
         queries = _copy_for_one_shot(queries, "queries", True)
     out = _check_out(out, queries, dev)
+    if tree is not None:
+        _check_tree_call(tree, B, L, S, window, causal, kernel, dev)
+        nbytes, _ = _tree_sizes(B, Hq, Hkv, L, D, S, int(group_size), int(window))
+        if nbytes == 0:
+            raise NotImplementedError(f"tree attention does not support B={B} Hq={Hq} Hkv={Hkv} L={L} D={D} S={S}")
+        stream = _lib.stream_ptr(dev)
+        qr, orr = _lib.rows(queries), _lib.rows(out)
+        kq = _lib.qtensor(*k_pool, range_exp=range_word(k_pool[0]))
+        vq = _lib.qtensor(*v_pool, range_exp=range_word(v_pool[0]))
+        with _on_device(dev):
+            ws = _tree_workspace(dev, stream, nbytes, workspace)
+            rc = _lib.lib().kvq_paged_tree_attn(
+                ctypes.byref(qr), ctypes.byref(kq), ctypes.byref(vq), k_pool[0].shape[0], block_tables.data_ptr(),
+                block_tables.stride(0), seq_lens.data_ptr(), ctypes.byref(orr), B, Hq, Hkv, L, D, S, int(bits),
+                int(group_size), _lib.dtype_code(queries.dtype), float(scale), ctypes.byref(tree.desc), int(window),
+                ws.data_ptr(), ws.numel() * ws.element_size(), stream)
+        _lib.check(rc, "kvq_paged_tree_attn")
+        return out
+    if workspace is not None:
+        raise ValueError("a workspace of the caller's is taken with tree= only")
     if kernel == "auto":
         kernel = _auto_kernel((Hq // Hkv) * L, D, group_size, dense=False, units=B * Hkv,
                               keys=min(S, window + L) if window else S)

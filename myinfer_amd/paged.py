@@ -183,10 +183,10 @@ class PagedRadixKVCache:
 
     def attention(self, layer: int, queries: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                   scale: float, *, causal: bool = False, window: int = 0, max_len: Optional[int] = None,
-                  kernel: str = "auto") -> torch.Tensor:
+                  kernel: str = "auto", tree: Optional[kernels.DraftTree] = None) -> torch.Tensor:
         return kernels.paged_attention(queries, self._k[layer], self._v[layer], block_tables, seq_lens, scale,
                                        causal=causal, window=window, group_size=self.group_size, bits=self.bits,
-                                       max_len=max_len, kernel=kernel)
+                                       max_len=max_len, kernel=kernel, tree=tree)
 
     def gather(self, layer: int, block_table: Sequence[int], length: int):
         """The first `length` rows of one sequence as contiguous [1, Hkv, length, *] triples (K, V)."""
