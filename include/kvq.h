@@ -137,6 +137,48 @@ int kvq_rope_quantize_append(const kvq_rows* k_src, const kvq_qtensor* k_dst,
                              int64_t row_offset, int B, int H, int L, int D,
                              int bits, int group_size, int dtype, void* stream);
 
+/* Rotary embedding at positions given per row, over 1 to KVQ_MAX_AXES axes (time, height, width of an image or
+ * video token; the depth of a drafted token). Pair i turns by positions[axis(i)][b][l] * scale * freq(i), formed
+ * and reduced in double precision, rotated in fp32 and rounded to T. (kvq_rope forms its angles in fp32: the two
+ * agree to an ulp of T at near positions, not at far ones, where this one's are the exact ones.) No counterpart
+ * in the reference. */
+#define KVQ_MAX_AXES 4
+typedef struct kvq_axes {
+  int dims;        /* rotated leading dims, as in kvq_rope_params                                           */
+  int traditional; /* 0: pairs (i, i + dims/2); 1: pairs (2i, 2i + 1)                                       */
+  int axes;        /* position axes                                                                         */
+  int sections[KVQ_MAX_AXES]; /* pairs of each axis, at least 1 each, dims/2 in all                         */
+  int interleaved; /* 0: the first sections[0] pairs belong to axis 0, the next to axis 1, ...; 1: pairs are
+                      dealt to the axes in turn, passing over those that have all of theirs                 */
+  int restart;     /* 0: freq(i) = base^(-2 i / dims); 1: every axis counts its own pairs, base^(-j / sections[a])
+                      for its pair j                                                                        */
+  double base, scale;
+  const int32_t* positions; /* device int32 [axes][B][L]; strides in elements, 0 broadcasts                 */
+  int64_t pos_stride_a, pos_stride_b, pos_stride_l;
+} kvq_axes;
+
+/* In-place rotation of rows [0, L) of x (T[B][H][L][D]) by `rope`. */
+int kvq_rope_axes(const kvq_rows* x, const kvq_axes* rope, int B, int H, int L, int D, int dtype, void* stream);
+
+/*
+ * kvq_rope_quantize_append with `rope`'s positions, in one launch with the rotation of the step's queries: the
+ * keys are rotated, rounded to T and quantized, the values quantized, and the rows of q (T[B][Hq][L][D]; NULL: none,
+ * Hq is then not read) rotated in place. block_table NULL: into rows [row_offset, row_offset + L) of a
+ * contiguous cache (starts must be NULL); else into pages as kvq_paged_quantize_append does.
+ */
+int kvq_rope_axes_append(const kvq_rows* k_src, const kvq_qtensor* k_dst, const kvq_rows* v_src,
+                         const kvq_qtensor* v_dst, const kvq_rows* q, int Hq, const kvq_axes* rope, int num_pages,
+                         const int32_t* block_table, int64_t table_stride, const int32_t* starts, int64_t row_offset,
+                         int B, int H, int L, int D, int bits, int group_size, int dtype, void* stream);
+
+/*
+ * Rows [row_offset, row_offset + L) of a quantized K (and V, when not NULL) read back as values, scale * code +
+ * bias rounded to T, into rows [0, L) of k_dst (and v_dst), in one launch. Replaces: mx.dequantize. Support and
+ * alignment as kvq_quantize_append (the destination rows as its sources).
+ */
+int kvq_dequantize(const kvq_qtensor* k_src, const kvq_rows* k_dst, const kvq_qtensor* v_src, const kvq_rows* v_dst,
+                   int64_t row_offset, int B, int H, int L, int D, int bits, int group_size, int dtype, void* stream);
+
 /*
  * Attention of L query rows per sequence against a quantized cache, for small L (decode):
  * out = softmax(scale * q K^T + mask) V over the dequantized K/V.
@@ -372,6 +414,38 @@ int kvq_paged_quantize_append(const kvq_rows* k_src, const kvq_qtensor* k_pool,
                               const int32_t* block_table, int64_t table_stride, const int32_t* starts,
                               int64_t row_offset, const kvq_rope_params* rope,
                               int B, int H, int L, int D, int bits, int group_size, int dtype, void* stream);
+
+/*
+ * kvq_dequantize from paged pools: rows [0, min(L, seq_lens[b])) of sequence b into the same rows of k_dst (and
+ * v_dst); its rows behind that are left as they are. table_stride >= ceil(L / KVQ_PAGE_ROWS); table entries are
+ * clamped to the pool.
+ */
+int kvq_paged_dequantize(const kvq_qtensor* k_pool, const kvq_rows* k_dst, const kvq_qtensor* v_pool, const kvq_rows* v_dst,
+                         int num_pages, const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens,
+                         int B, int H, int L, int D, int bits, int group_size, int dtype, void* stream);
+
+/* An array of rows [B][H][rows][row_bytes] whose rows may be moved: codes, scales or biases of a cache, or the K or
+ * V of an unquantized one; of a paged pool stride_b is the page stride. Strides in bytes, all of them, row_bytes
+ * and the address even. */
+typedef struct kvq_row_array {
+  void* data;
+  int64_t stride_b, stride_h, stride_l, row_bytes;
+} kvq_row_array;
+
+/*
+ * The accepted rows of drafted ones move up, in place and in every array (all layers' in one launch per 192
+ * arrays): row start + i of sequence b becomes what row start + rows[b][i] held before the call, for i < M. rows:
+ * device int32 [B][M] (batch stride rows_stride_b, 0: one list for all), indices among the n rows from `start`.
+ * An entry outside [i, n) leaves row start + i as it is (an ascending list, such as an accepted path, has none but
+ * padding of -1 at its end). Rows from start + M on are not written.
+ * block_table NULL: contiguous arrays, rows [start, start + n) of each (starts must be NULL). Else paged pools,
+ * start of sequence b starts[b] (device int32 [B], or NULL: `start`); a row whose page is outside the table, or whose
+ * entry is outside [0, num_pages), is neither read nor written. The pages moved into must belong to one sequence.
+ * M <= n; B <= 65535.
+ */
+int kvq_keep_rows(const kvq_row_array* arrays, int n_arrays, int num_pages, const int32_t* block_table,
+                  int64_t table_stride, const int32_t* rows, int64_t rows_stride_b, const int32_t* starts, int64_t start,
+                  int n, int M, int B, int H, void* stream);
 
 /*
  * kvq_decode_attn / kvq_prefill_attn over paged pools (same arguments, masks, workspace sizes and

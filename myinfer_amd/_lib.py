@@ -62,6 +62,24 @@ class RopeParams(ctypes.Structure):
                 ("offset", c_int64)]
 
 
+MAX_AXES = 4  # KVQ_MAX_AXES
+
+
+class Axes(ctypes.Structure):
+    """kvq_axes: rotary embedding at int32 positions [axes][B][L]."""
+
+    _fields_ = [("dims", c_int), ("traditional", c_int), ("axes", c_int), ("sections", c_int * MAX_AXES),
+                ("interleaved", c_int), ("restart", c_int), ("base", ctypes.c_double), ("scale", ctypes.c_double),
+                ("positions", c_void_p), ("pos_stride_a", c_int64), ("pos_stride_b", c_int64), ("pos_stride_l", c_int64)]
+
+
+class RowArray(ctypes.Structure):
+    """kvq_row_array: rows [B][H][rows][row_bytes] that kvq_keep_rows moves (strides in bytes)."""
+
+    _fields_ = [("data", c_void_p), ("stride_b", c_int64), ("stride_h", c_int64), ("stride_l", c_int64),
+                ("row_bytes", c_int64)]
+
+
 _ATTN_ARGS = [
     POINTER(Rows), POINTER(QTensor), POINTER(QTensor), c_void_p, POINTER(Rows),
     c_int, c_int, c_int, c_int, c_int, c_int,  # B Hq Hkv L D S
@@ -160,6 +178,27 @@ SIGNATURES = {
     ),
     "kvq_paged_decode_attn": (c_int, _PAGED_ATTN_ARGS),
     "kvq_paged_prefill_attn": (c_int, _PAGED_ATTN_ARGS),
+    "kvq_rope_axes": (c_int, [POINTER(Rows), POINTER(Axes), c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "kvq_rope_axes_append": (
+        c_int,
+        [POINTER(Rows), POINTER(QTensor), POINTER(Rows), POINTER(QTensor), POINTER(Rows), c_int, POINTER(Axes),
+         c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    ),
+    "kvq_dequantize": (
+        c_int,
+        [POINTER(QTensor), POINTER(Rows), POINTER(QTensor), POINTER(Rows), c_int64,
+         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    ),
+    "kvq_paged_dequantize": (
+        c_int,
+        [POINTER(QTensor), POINTER(Rows), POINTER(QTensor), POINTER(Rows), c_int, c_void_p, c_int64, c_void_p,
+         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    ),
+    "kvq_keep_rows": (
+        c_int,
+        [POINTER(RowArray), c_int, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+         c_int, c_int, c_int, c_int, c_void_p],
+    ),
     "kvq_draft_tree": (
         c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
     ),

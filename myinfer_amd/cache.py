@@ -302,12 +302,19 @@ class QuantizedKVCache:
         if self.keys is None or self.keys[0].shape[2] < capacity:
             self._resize(like, like, 0, capacity=capacity)
 
-    def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor, rope: Optional["kernels.Rope"] = None):
+    def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor, rope=None,
+                         positions: Optional[torch.Tensor] = None, queries: Optional[torch.Tensor] = None):
         """Append keys/values [B, H, L, D] at `offset` and return the fetched views. With `rope`,
         the keys are rotated (positions offset .. offset + L - 1) in the same launch that
-        quantizes them: the RoPE + cache update an attention layer does, fused."""
+        quantizes them: the RoPE + cache update an attention layer does, fused. With a
+        ``kernels.RopeAxes`` they are rotated at `positions` (int32 [axes, B, L] or [axes, L]), and the
+        rows of `queries` [B, Hq, L, D], if given, in place in that launch too."""
         prev = self.offset
         L = keys.shape[2]
+        if isinstance(rope, kernels.RopeAxes):
+            return self._update_axes(keys, values, rope, positions, queries)
+        if positions is not None or queries is not None:
+            raise ValueError("positions and queries go with a kernels.RopeAxes")
         if self.keys is None or prev + L > self.keys[0].shape[2]:
             self._resize(keys, values, L)
         # the append's descriptors are built once per buffer set, RoPE and stream
@@ -319,6 +326,62 @@ class QuantizedKVCache:
         self._append(keys, values, prev)
         self.offset += L
         return self.fetch()
+
+    def _update_axes(self, keys, values, rope, positions, queries):
+        if positions is None:
+            raise ValueError("a kernels.RopeAxes needs positions")
+        prev, L = self.offset, keys.shape[2]
+        if self.keys is None or prev + L > self.keys[0].shape[2]:
+            self._resize(keys, values, L)
+        key = (id(self.keys[0]), id(self.values[0]), rope)
+        if getattr(self, "_axes_key", None) != key:
+            self._axes = kernels.prepare_axes_append(self.keys, self.values, rope=rope, group_size=self.group_size,
+                                                     bits=self.bits)
+            self._axes_key = key
+        self._axes(keys, values, positions, prev, queries)
+        self.offset += L
+        return self.fetch()
+
+    def restore(self, keys, values, rows: int) -> None:
+        """Take over buffers that hold a saved cache: K and V (codes, scales, biases) triples [B, H, cap, *] of which the
+        first `rows` are cached rows (later appends write behind them, and grow the cache when they are full)."""
+        for name, tr in (("keys", keys), ("values", values)):
+            if len(tr) != 3 or any(x.dim() != 4 for x in tr) or any(x.shape[:3] != tr[0].shape[:3] for x in tr):
+                raise ValueError(f"{name} must be a (codes, scales, biases) triple [B, H, cap, *]")
+            if tr[0].shape[3] * 32 != tr[1].shape[3] * self.group_size * self.bits or tr[1].shape != tr[2].shape:
+                raise ValueError(f"{name}: row widths do not match {self.bits} bits and group_size {self.group_size}")
+            if tr[1].dtype != keys[1].dtype or tr[0].dtype != torch.uint32 or tr[0].shape[:3] != keys[0].shape[:3]:
+                raise ValueError("codes are uint32, and keys and values share their rows and dtype")
+        if not 0 <= rows <= keys[0].shape[2]:
+            raise ValueError(f"{rows} rows in buffers of {keys[0].shape[2]}")
+        words = [kernels.range_exponent(tuple(x[:, :, :rows] for x in tr), self.bits) for tr in (keys, values)]
+        self.keys, self.values, self.offset = tuple(keys), tuple(values), int(rows)
+        self.range_exp = torch.cat(words)
+        kernels.register_range_word(self.keys[0], self.range_exp[0:1])
+        kernels.register_range_word(self.values[0], self.range_exp[1:2])
+
+    def dequantized(self, start: int = 0, stop: Optional[int] = None):
+        """Rows [start, stop) (default: all) read back as values: K and V [B, H, n, D] in their dtype, one launch."""
+        stop = self.offset if stop is None else stop
+        if self.keys is None or not 0 <= start <= stop <= self.offset:
+            raise ValueError(f"rows [{start}, {stop}) of a cache of {self.offset}")
+        return kernels.dequantize_rows(tuple(x[:, :, start:stop] for x in self.keys),
+                                       tuple(x[:, :, start:stop] for x in self.values), group_size=self.group_size,
+                                       bits=self.bits)
+
+    def to_unquantized(self) -> KVCache:
+        """The cached rows as a plain KVCache: the way back from ``KVCache.to_quantized``."""
+        out = KVCache()
+        out.offset = self.offset
+        if self.keys is not None:
+            B, H, cap = self.keys[0].shape[:3]
+            D = self.keys[1].shape[3] * self.group_size
+            out.keys, out.values = (torch.zeros((B, H, cap, D), dtype=self.keys[1].dtype, device=self.keys[1].device)
+                                    for _ in range(2))
+            o = self.offset
+            kernels.dequantize_rows(tuple(x[:, :, :o] for x in self.keys), tuple(x[:, :, :o] for x in self.values),
+                                    group_size=self.group_size, bits=self.bits, out=(out.keys[:, :, :o], out.values[:, :, :o]))
+        return out
 
     def fetch(self):
         """The (codes, scales, biases) views of the first `offset` rows, for K and for V."""
@@ -370,6 +433,32 @@ class QuantizedKVCache:
             return True
         keys, values = self.fetch()
         return kernels.fits_fp16_operands(keys, self.bits) and kernels.fits_fp16_operands(values, self.bits)
+
+
+def keep_rows(cache: List, start: int, rows: torch.Tensor) -> int:
+    """After the rows from `start` on were drafted and verified: keep those that `rows` names (int32 [B, M] or [M] on
+    the GPU, indices from `start` in ascending order, the accepted path of a tree), move them up to rows start ..
+    start + M - 1 in every layer's cache, and drop the rest, as ``trim_prompt_cache`` drops a rejected tail. One
+    launch for up to 32 layers. The caches are KVCache or QuantizedKVCache at one offset; returns the new one."""
+    if not cache:
+        raise ValueError("no caches")
+    if not torch.is_tensor(rows):
+        raise ValueError("rows must be an int32 tensor on the caches' device")
+    end = cache[0].offset
+    tensors = []
+    for c in cache:
+        if type(c) not in (KVCache, QuantizedKVCache):
+            raise ValueError(f"rows of a {type(c).__name__} are not kept by index")
+        if c.keys is None or c.offset != end:
+            raise ValueError("the caches must hold rows, all at one offset")
+        tensors += [c.keys, c.values] if type(c) is KVCache else [*c.keys, *c.values]
+    M = rows.shape[-1] if rows.dim() else 0
+    if not 0 <= start <= end or M > end - start:
+        raise ValueError(f"{M} rows cannot be kept of rows [{start}, {end})")
+    kernels.keep_rows(tensors, rows, start, end - start)
+    for c in cache:
+        c.offset = start + M
+    return start + M
 
 
 def can_trim_prompt_cache(cache: List) -> bool:

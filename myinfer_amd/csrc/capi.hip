@@ -181,7 +181,7 @@ int check_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, co
 }
 
 int check_quantize(const kvq_rows* k_src, const kvq_qtensor* k_dst, const kvq_rows* v_src, const kvq_qtensor* v_dst,
-                   int64_t row_offset, int B, int H, int L, int D, int bits, int group_size, int dtype) {
+                   int64_t row_offset, int B, int H, int L, int D, int bits, int group_size, int dtype, bool read = false) {
   int rc;
   if ((rc = check_dtype(dtype))) return rc;
   if (bits != 2 && bits != 4 && bits != 8) return fail(KVQ_ERR_UNSUPPORTED, "bits must be 2, 4 or 8, got %d", bits);
@@ -190,12 +190,14 @@ int check_quantize(const kvq_rows* k_src, const kvq_qtensor* k_dst, const kvq_ro
   if (B < 0 || H < 0 || L < 0 || D <= 0) return fail(KVQ_ERR_INVALID, "negative shape (B=%d H=%d L=%d D=%d)", B, H, L, D);
   if (D % group_size) return fail(KVQ_ERR_INVALID, "D=%d is not a multiple of group_size=%d", D, group_size);
   if (row_offset < 0) return fail(KVQ_ERR_INVALID, "row_offset must be >= 0");
+  // (reading back, the rows are the destination)
+  const char *kr = read ? "k_dst" : "k_src", *kq = read ? "k_src" : "k_dst", *vr = read ? "v_dst" : "v_src", *vq = read ? "v_src" : "v_dst";
   if ((v_src == nullptr) != (v_dst == nullptr)) return fail(KVQ_ERR_INVALID, "v_src and v_dst must both be given or both be NULL");
-  if ((rc = check_rows(k_src, "k_src", D, true))) return rc;
-  if ((rc = check_qtensor(k_dst, "k_dst"))) return rc;
+  if ((rc = check_rows(k_src, kr, D, true))) return rc;
+  if ((rc = check_qtensor(k_dst, kq))) return rc;
   if (v_src) {
-    if ((rc = check_rows(v_src, "v_src", D, true))) return rc;
-    if ((rc = check_qtensor(v_dst, "v_dst"))) return rc;
+    if ((rc = check_rows(v_src, vr, D, true))) return rc;
+    if ((rc = check_qtensor(v_dst, vq))) return rc;
   }
   const int64_t row_words = (int64_t)D * bits / 32;
   for (const kvq_qtensor* t : {k_dst, v_dst}) {
@@ -277,6 +279,28 @@ int check_rope(const kvq_rope_params* r, int D) {
   return KVQ_OK;
 }
 
+int check_axes(const kvq_axes* r, int D) {
+  if (!r) return fail(KVQ_ERR_INVALID, "rope descriptor is NULL");
+  if (r->dims <= 0 || r->dims > D || r->dims > 256 || r->dims % 16)
+    return fail(KVQ_ERR_UNSUPPORTED, "rope dims must be a positive multiple of 16, at most D=%d and 256, got %d", D,
+                r->dims);
+  if (r->axes < 1 || r->axes > KVQ_MAX_AXES)
+    return fail(KVQ_ERR_UNSUPPORTED, "rope needs 1 to %d position axes, got %d", KVQ_MAX_AXES, r->axes);
+  int64_t pairs = 0;
+  for (int a = 0; a < r->axes; ++a) {
+    if (r->sections[a] < 1) return fail(KVQ_ERR_INVALID, "rope section %d has %d pairs: at least 1 is needed", a, r->sections[a]);
+    pairs += r->sections[a];
+  }
+  if (pairs != r->dims / 2)
+    return fail(KVQ_ERR_INVALID, "rope sections hold %lld pairs, dims %d have %d", (long long)pairs, r->dims, r->dims / 2);
+  if (!(r->base > 0.0) || !isfinite(r->base)) return fail(KVQ_ERR_INVALID, "rope base must be positive and finite");
+  if (!isfinite(r->scale)) return fail(KVQ_ERR_INVALID, "rope scale is not finite");
+  if (!r->positions) return fail(KVQ_ERR_INVALID, "rope positions are NULL");
+  if (!aligned(r->positions, 4) || r->pos_stride_a < 0 || r->pos_stride_b < 0 || r->pos_stride_l < 0)
+    return fail(KVQ_ERR_INVALID, "rope positions must be 4-byte aligned with non-negative strides");
+  return KVQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -334,6 +358,99 @@ int kvq_paged_quantize_append(const kvq_rows* k_src, const kvq_qtensor* k_pool, 
                                                       starts, row_offset, rope, B, H, L, D, bits, group_size, dtype,
                                                       (hipStream_t)stream),
                     "paged_quantize_append launch");
+}
+
+int kvq_rope_axes(const kvq_rows* x, const kvq_axes* rope, int B, int H, int L, int D, int dtype, void* stream) {
+  int rc;
+  if ((rc = check_dtype(dtype))) return rc;
+  if (B < 0 || H < 0 || L < 0 || D <= 0 || D % 8) return fail(KVQ_ERR_INVALID, "bad shape (B=%d H=%d L=%d D=%d)", B, H, L, D);
+  if ((rc = check_axes(rope, D))) return rc;
+  if ((rc = check_rows(x, "x", D, true))) return rc;
+  if (B == 0 || H == 0 || L == 0) return ok();
+  return hip_status(kvq::launch_rope_axes(x, rope, B, H, L, dtype, (hipStream_t)stream), "rope_axes launch");
+}
+
+int kvq_rope_axes_append(const kvq_rows* k_src, const kvq_qtensor* k_dst, const kvq_rows* v_src, const kvq_qtensor* v_dst,
+                         const kvq_rows* q, int Hq, const kvq_axes* rope, int num_pages, const int32_t* block_table,
+                         int64_t table_stride, const int32_t* starts, int64_t row_offset, int B, int H, int L, int D,
+                         int bits, int group_size, int dtype, void* stream) {
+  int rc;
+  if ((rc = check_axes(rope, D))) return rc;
+  if ((rc = check_quantize(k_src, k_dst, v_src, v_dst, row_offset, B, H, L, D, bits, group_size, dtype))) return rc;
+  if (q) {
+    if (Hq < 0) return fail(KVQ_ERR_INVALID, "negative shape (Hq=%d)", Hq);
+    if ((rc = check_rows(q, "queries", D, true))) return rc;
+  }
+  if (block_table) {
+    if ((rc = check_pool(k_dst, "k_pool", H, D, bits, group_size, num_pages))) return rc;
+    if (v_dst && (rc = check_pool(v_dst, "v_pool", H, D, bits, group_size, num_pages))) return rc;
+    if ((rc = check_table(block_table, table_stride, starts ? 1 : row_offset + L))) return rc;
+  } else if (starts) {
+    return fail(KVQ_ERR_INVALID, "starts need a block table");
+  }
+  if (B == 0 || L == 0 || H == 0) return ok();
+  return hip_status(kvq::launch_rope_axes_append(k_src, k_dst, v_src, v_dst, Hq > 0 ? q : nullptr, Hq, rope, num_pages,
+                                                 block_table, table_stride, starts, row_offset, B, H, L, D, bits, group_size,
+                                                 dtype, (hipStream_t)stream),
+                    "rope_axes_append launch");
+}
+
+int kvq_dequantize(const kvq_qtensor* k_src, const kvq_rows* k_dst, const kvq_qtensor* v_src, const kvq_rows* v_dst,
+                   int64_t row_offset, int B, int H, int L, int D, int bits, int group_size, int dtype, void* stream) {
+  int rc;
+  if ((rc = check_quantize(k_dst, k_src, v_dst, v_src, row_offset, B, H, L, D, bits, group_size, dtype, true))) return rc;
+  if (B == 0 || H == 0 || L == 0) return ok();
+  return hip_status(kvq::launch_dequantize(k_src, k_dst, v_src, v_dst, 0, nullptr, 0, nullptr, row_offset, B, H, L, D, bits,
+                                           group_size, dtype, (hipStream_t)stream),
+                    "dequantize launch");
+}
+
+int kvq_paged_dequantize(const kvq_qtensor* k_pool, const kvq_rows* k_dst, const kvq_qtensor* v_pool, const kvq_rows* v_dst,
+                         int num_pages, const int32_t* block_table, int64_t table_stride, const int32_t* seq_lens, int B,
+                         int H, int L, int D, int bits, int group_size, int dtype, void* stream) {
+  int rc;
+  if ((rc = check_quantize(k_dst, k_pool, v_dst, v_pool, 0, B, H, L, D, bits, group_size, dtype, true))) return rc;
+  if ((rc = check_pool(k_pool, "k_pool", H, D, bits, group_size, num_pages))) return rc;
+  if (v_pool && (rc = check_pool(v_pool, "v_pool", H, D, bits, group_size, num_pages))) return rc;
+  if ((rc = check_table(block_table, table_stride, L))) return rc;
+  if (!seq_lens) return fail(KVQ_ERR_INVALID, "seq_lens is NULL");
+  if (B == 0 || H == 0 || L == 0) return ok();
+  return hip_status(kvq::launch_dequantize(k_pool, k_dst, v_pool, v_dst, num_pages, block_table, table_stride, seq_lens, 0, B,
+                                           H, L, D, bits, group_size, dtype, (hipStream_t)stream),
+                    "paged_dequantize launch");
+}
+
+int kvq_keep_rows(const kvq_row_array* arrays, int n_arrays, int num_pages, const int32_t* block_table, int64_t table_stride,
+                  const int32_t* rows, int64_t rows_stride_b, const int32_t* starts, int64_t start, int n, int M, int B,
+                  int H, void* stream) {
+  if (n_arrays < 0 || n < 0 || M < 0 || B < 0 || H < 0)
+    return fail(KVQ_ERR_INVALID, "negative shape (arrays=%d n=%d M=%d B=%d H=%d)", n_arrays, n, M, B, H);
+  if (M > n) return fail(KVQ_ERR_INVALID, "%d rows cannot be kept of %d", M, n);
+  if (B > 65535) return fail(KVQ_ERR_UNSUPPORTED, "a batch of at most 65535, got %d", B);
+  if (n_arrays > 0 && !arrays) return fail(KVQ_ERR_INVALID, "arrays is NULL");
+  if (!rows || !aligned(rows, 4) || !aligned(starts, 4) || rows_stride_b < 0)
+    return fail(KVQ_ERR_INVALID, "rows must not be NULL, rows and starts 4-byte aligned, with a non-negative batch stride");
+  if (start < 0) return fail(KVQ_ERR_INVALID, "start must be >= 0");
+  if (block_table) {
+    if (!aligned(block_table, 4) || table_stride <= 0 || num_pages <= 0)
+      return fail(KVQ_ERR_INVALID, "block_table must be 4-byte aligned, table_stride and num_pages positive");
+  } else if (starts) {
+    return fail(KVQ_ERR_INVALID, "starts need a block table");
+  }
+  for (int i = 0; i < n_arrays; ++i) {
+    const kvq_row_array& a = arrays[i];
+    if (!a.data) return fail(KVQ_ERR_INVALID, "array %d has a NULL pointer", i);
+    if (a.stride_b < 0 || a.stride_h < 0 || a.stride_l <= 0 || a.row_bytes <= 0)
+      return fail(KVQ_ERR_INVALID, "array %d has a negative or zero stride or width", i);
+    if (!aligned(a.data, 2) || (a.stride_b | a.stride_h | a.stride_l | a.row_bytes) & 1)
+      return fail(KVQ_ERR_INVALID, "array %d has an odd address, stride or width", i);
+    if (a.stride_l < a.row_bytes || a.row_bytes > 65536)
+      return fail(KVQ_ERR_INVALID, "array %d: rows of %lld bytes every %lld", i, (long long)a.row_bytes, (long long)a.stride_l);
+  }
+  if (n_arrays == 0 || M == 0 || B == 0 || H == 0) return ok();
+  return hip_status(kvq::launch_keep_rows(arrays, n_arrays, num_pages, block_table, table_stride, rows, rows_stride_b, starts,
+                                          start, n, M, B, H, (hipStream_t)stream),
+                    "keep_rows launch");
 }
 
 size_t kvq_decode_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window) {

@@ -82,6 +82,20 @@ hipError_t launch_prefill_dense(const kvq_rows* q, const kvq_rows* k, const kvq_
                                 const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype,
                                 float scale, int causal, int window, void* workspace, hipStream_t stream,
                                 const kvq_tree* tree = nullptr);
+// rope_axes.hip: rotation at positions of several axes, alone and with the append (table null: a contiguous cache)
+hipError_t launch_rope_axes(const kvq_rows* x, const kvq_axes* rope, int B, int H, int L, int dtype, hipStream_t stream);
+hipError_t launch_rope_axes_append(const kvq_rows* k_src, const kvq_qtensor* k_dst, const kvq_rows* v_src,
+                                   const kvq_qtensor* v_dst, const kvq_rows* q, int Hq, const kvq_axes* rope, int num_pages,
+                                   const int32_t* table, int64_t table_stride, const int32_t* starts, int64_t row_offset,
+                                   int B, int H, int L, int D, int bits, int G, int dtype, hipStream_t stream);
+// dequantize.hip: rows [row0, row0 + L) read back (v_src null: one tensor; lens null: a contiguous cache)
+hipError_t launch_dequantize(const kvq_qtensor* k_src, const kvq_rows* k_dst, const kvq_qtensor* v_src, const kvq_rows* v_dst,
+                             int num_pages, const int32_t* table, int64_t table_stride, const int32_t* lens, int64_t row0,
+                             int B, int H, int64_t L, int D, int bits, int G, int dtype, hipStream_t stream);
+// keep.hip: rows moved up in place (table null: contiguous arrays)
+hipError_t launch_keep_rows(const kvq_row_array* arrays, int n_arrays, int num_pages, const int32_t* table,
+                            int64_t table_stride, const int32_t* rows, int64_t rows_sb, const int32_t* starts, int64_t start,
+                            int n, int M, int B, int H, hipStream_t stream);
 // tree.hip: the bits and depths of a tree (kvq_draft_tree)
 hipError_t launch_draft_tree(const int32_t* parents, int64_t parents_sb, int B, int L, uint32_t* bits, int32_t* depths,
                              const int32_t* starts, int64_t start, int32_t* positions, hipStream_t stream);

@@ -140,6 +140,151 @@ def rope(x: torch.Tensor, r: Rope, offset: int = 0) -> torch.Tensor:
     return x
 
 
+@dataclass(frozen=True)
+class RopeAxes:
+    """Rotary position embedding at positions given per row, over 1 to 4 axes: the time, height and width of an
+    image's or a video's tokens, or one axis for rows that are not consecutive (a tree of drafted tokens). Pair i
+    of a row turns by position[axis(i)] * scale * freq(i).
+
+    ``sections``: pairs of each axis, dims / 2 in all (default: one axis). ``interleaved``: False: the first
+    sections[0] pairs belong to axis 0, the next sections[1] to axis 1, ...; True: pairs are dealt to the axes in turn,
+    passing over those that have all of theirs. ``restart``: False: freq(i) = base^(-2 i / dims); True: every axis
+    counts its own pairs, base^(-j / sections[axis]) for its pair j. ``traditional`` as in Rope.
+
+    Angles are formed and reduced in double precision (Rope's in fp32, as mlx's are: the two agree to an ulp of the
+    rows' type at near positions, and part at far ones)."""
+
+    dims: int
+    sections: Tuple[int, ...] = ()
+    traditional: bool = False
+    base: float = 10000.0
+    scale: float = 1.0
+    interleaved: bool = False
+    restart: bool = False
+
+    def __post_init__(self):
+        sections = tuple(int(n) for n in self.sections) or (int(self.dims) // 2,)
+        if not 1 <= len(sections) <= _lib.MAX_AXES:
+            raise ValueError(f"1 to {_lib.MAX_AXES} axes, got sections {sections}")
+        if min(sections) < 1 or sum(sections) != int(self.dims) // 2:
+            raise ValueError(f"sections {sections} must be at least 1 each and dims / 2 = {int(self.dims) // 2} in all")
+        object.__setattr__(self, "sections", sections)
+
+    @property
+    def axes(self) -> int:
+        return len(self.sections)
+
+    def params(self) -> "_lib.Axes":
+        """The descriptor without positions (``set_positions``)."""
+        return _lib.Axes(int(self.dims), int(bool(self.traditional)), self.axes, (ctypes.c_int * _lib.MAX_AXES)(*self.sections),
+                         int(bool(self.interleaved)), int(bool(self.restart)), float(self.base), float(self.scale), None, 0, 0, 0)
+
+
+def _set_positions(desc: "_lib.Axes", positions: torch.Tensor, B: int, L: int, dev: torch.device) -> None:
+    """Point `desc` at int32 positions [axes, B, L] (or [axes, L], the same for every sequence) after their checks."""
+    A = desc.axes
+    if not torch.is_tensor(positions) or positions.dtype != torch.int32 or positions.device != dev:
+        raise ValueError(f"positions must be an int32 tensor on {dev}")
+    if tuple(positions.shape) == (A, B, L):
+        sa, sb, sl = positions.stride()
+    elif tuple(positions.shape) == (A, L):
+        (sa, sl), sb = positions.stride(), 0
+    else:
+        raise ValueError(f"positions must be [axes, B, L] = {(A, B, L)} or [axes, L], got {tuple(positions.shape)}")
+    desc.positions, desc.pos_stride_a, desc.pos_stride_b, desc.pos_stride_l = positions.data_ptr(), sa, sb, sl
+
+
+def rope_axes(x: torch.Tensor, r: RopeAxes, positions: torch.Tensor) -> torch.Tensor:
+    """Rotate x [B, H, L, D] (float16/bfloat16, CUDA) in place, row l of sequence b at positions[:, b, l], and return
+    it. positions: int32 [axes, B, L] or [axes, L]."""
+    dev = _require_cuda(x)
+    if x.dim() != 4:
+        raise ValueError(f"x must be [B, H, L, D], got {tuple(x.shape)}")
+    B, H, L, D = x.shape
+    xr, rp = _lib.rows(x), r.params()
+    _set_positions(rp, positions, B, L, dev)
+    if x.numel() == 0:
+        return x
+    with _on_device(dev):
+        rc = _lib.lib().kvq_rope_axes(ctypes.byref(xr), ctypes.byref(rp), B, H, L, D, _lib.dtype_code(x.dtype),
+                                      _lib.stream_ptr(dev))
+    _lib.check(rc, "kvq_rope_axes")
+    return x
+
+
+class AxesAppendCall:
+    """A quantize-append into fixed destination buffers, with the rotation of the step's keys and queries at given
+    positions, its descriptors built once (``prepare_axes_append``). Launches on the stream current at the call."""
+
+    def __init__(self, k_dst: Triple, v_dst: Optional[Triple], rope: RopeAxes, group_size: int, bits: int):
+        _check_triple(k_dst, "k_dst")
+        tens = list(k_dst)
+        if v_dst is not None:
+            _check_triple(v_dst, "v_dst")
+            tens += list(v_dst)
+            if any(tuple(a.shape) != tuple(b.shape) for a, b in zip(k_dst, v_dst)) or v_dst[1].dtype != k_dst[1].dtype:
+                raise ValueError("k_dst and v_dst must have the same shapes and dtype")
+        self._dev = _require_cuda(*tens)
+        self._keep = (k_dst, v_dst)
+        codes, scales, _ = k_dst
+        if tuple(scales.shape[:3]) != tuple(codes.shape[:3]):
+            raise ValueError("the destination's codes and scales must have the same rows")
+        self._lead, self._rows = tuple(codes.shape[:2]), codes.shape[2]
+        self._widths = (codes.shape[3], scales.shape[3])
+        self._kq = _lib.qtensor(*k_dst, range_exp=range_word(k_dst[0]))
+        self._vq = None if v_dst is None else _lib.qtensor(*v_dst, range_exp=range_word(v_dst[0]))
+        self._dtype, self._code = scales.dtype, _lib.dtype_code(scales.dtype)
+        self._bits, self._group = int(bits), int(group_size)
+        self._rp = rope.params()
+
+    def _check(self, k, v, positions, queries) -> tuple:
+        if k.dtype != self._dtype or k.device != self._dev or k.dim() != 4:
+            raise ValueError(f"keys must be {self._dtype} [B, H, L, D] on {self._dev}")
+        B, H, L, D = k.shape
+        if self._widths != (D * self._bits // 32, D // self._group):
+            raise ValueError("destination row widths do not match D, bits and group_size")
+        if (v is None) != (self._vq is None) or (v is not None and (v.shape != k.shape or v.dtype != k.dtype or
+                                                                    v.device != self._dev)):
+            raise ValueError("values must match the keys and a value destination")
+        if queries is not None and (queries.dtype != k.dtype or queries.device != self._dev or queries.dim() != 4 or
+                                    queries.shape[0] != B or tuple(queries.shape[2:]) != (L, D)):
+            raise ValueError(f"queries must be {self._dtype} [{B}, Hq, {L}, {D}] on {self._dev}")
+        rp = _lib.Axes.from_buffer_copy(self._rp)
+        _set_positions(rp, positions, B, L, self._dev)
+        return rp, B, H, L, D
+
+    def _launch(self, k, v, queries, rp, B, H, L, D, row_offset, paging) -> None:
+        if k.numel() == 0:
+            return
+        if queries is not None and queries.numel() == 0:
+            queries = None
+        kr = _lib.rows(k)
+        vr = None if v is None else _lib.rows(v)
+        qr = None if queries is None else _lib.rows(queries)
+        ref = ctypes.byref
+        with _on_device(self._dev):
+            rc = _lib.lib().kvq_rope_axes_append(
+                ref(kr), ref(self._kq), None if vr is None else ref(vr), None if vr is None else ref(self._vq),
+                None if qr is None else ref(qr), 0 if qr is None else queries.shape[1], ref(rp), *paging, int(row_offset), B, H,
+                L, D, self._bits, self._group, self._code, _lib.stream_ptr(self._dev))
+        _lib.check(rc, "kvq_rope_axes_append")
+
+    def __call__(self, k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, row_offset: int,
+                 queries: Optional[torch.Tensor] = None) -> None:
+        rp, B, H, L, D = self._check(k, v, positions, queries)
+        if (B, H) != self._lead:
+            raise ValueError(f"destination leads {self._lead} do not match source {(B, H)}")
+        if row_offset < 0 or row_offset + L > self._rows:
+            raise ValueError(f"rows [{row_offset}, {row_offset + L}) exceed the destination's {self._rows} rows")
+        self._launch(k, v, queries, rp, B, H, L, D, row_offset, (0, None, 0, None))
+
+
+def prepare_axes_append(k_dst: Triple, v_dst: Optional[Triple] = None, *, rope: RopeAxes, group_size: int = 64,
+                        bits: int = 8) -> AxesAppendCall:
+    """Build an ``AxesAppendCall`` for repeated appends into the same (codes, scales, biases) buffers."""
+    return AxesAppendCall(k_dst, v_dst, rope, group_size, bits)
+
+
 def quantize_append(k: torch.Tensor, k_dst: Triple, v: Optional[torch.Tensor] = None, v_dst: Optional[Triple] = None,
                     row_offset: int = 0, group_size: int = 64, bits: int = 8, rope: Optional[Rope] = None,
                     rope_offset: Optional[int] = None) -> None:
@@ -294,6 +439,61 @@ def quantize(x: torch.Tensor, group_size: int = 64, bits: int = 8) -> Triple:
     biases = torch.empty_like(scales)
     quantize_append(x4, (codes, scales, biases), row_offset=0, group_size=group_size, bits=bits)
     return (codes.reshape(*lead, -1), scales.reshape(*lead, -1), biases.reshape(*lead, -1))
+
+
+def _check_read(k: Triple, v: Optional[Triple], group_size: int, bits: int):
+    """The device, leading dims and head dim of triples to be read back, after their checks."""
+    tens = []
+    for name, tr in (("keys", k), ("values", v)):
+        if tr is None:
+            continue
+        _check_triple(tr, name)
+        if any(x.dim() != 4 for x in tr) or tr[1].shape[:3] != tr[0].shape[:3]:
+            raise ValueError(f"{name} must be 4-D (codes, scales, biases) with the same rows")
+        if tr[0].shape[3] * 32 // bits != tr[1].shape[3] * group_size:
+            raise ValueError(f"{name}: codes of {tr[0].shape[3]} words and {tr[1].shape[3]} groups are not rows of one "
+                             f"width at {bits} bits and group_size {group_size}")
+        if tuple(tr[0].shape) != tuple(k[0].shape) or tr[1].dtype != k[1].dtype:
+            raise ValueError("keys and values must have the same shapes and dtype")
+        tens += list(tr)
+    return _require_cuda(*tens), tuple(k[0].shape[:3]), k[1].shape[3] * group_size
+
+
+def _read_out(out, n: int, shape, dtype, dev, fresh):
+    if out is None:
+        return tuple(fresh(shape, dtype=dtype, device=dev) for _ in range(n))
+    out = tuple(out)
+    if len(out) != n or any(tuple(o.shape) != shape or o.dtype != dtype or o.device != dev for o in out):
+        raise ValueError(f"out must be {n} {dtype} tensors of shape {shape} on {dev}")
+    return out
+
+
+def dequantize_rows(k: Triple, v: Optional[Triple] = None, *, group_size: int = 64, bits: int = 8, out=None):
+    """The rows of quantized triples [B, H, S, *] (views of a cache) as values [B, H, S, D] in their dtype, K and V in
+    one launch: (K, V), or (K,) without v. `out`: the tensors to fill instead of new ones."""
+    dev, (B, H, S), D = _check_read(k, v, group_size, bits)
+    outs = _read_out(out, 1 if v is None else 2, (B, H, S, D), k[1].dtype, dev, torch.empty)
+    if outs[0].numel() == 0:
+        return outs
+    kq, kr = _lib.qtensor(*k), _lib.rows(outs[0])
+    vq, vr = (None, None) if v is None else (_lib.qtensor(*v), _lib.rows(outs[1]))
+    ref = ctypes.byref
+    with _on_device(dev):
+        rc = _lib.lib().kvq_dequantize(ref(kq), ref(kr), None if v is None else ref(vq), None if v is None else ref(vr), 0, B, H,
+                                       S, D, int(bits), int(group_size), _lib.dtype_code(k[1].dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "kvq_dequantize")
+    return outs
+
+
+def dequantize(codes: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = 64,
+               bits: int = 8) -> torch.Tensor:
+    """Counterpart of mx.dequantize(w, scales, biases, group_size, bits) on the GPU: codes uint32 [..., D*bits/32],
+    scales and biases [..., D/G] -> values [..., D] in the scales' dtype."""
+    if codes.shape[:-1] != scales.shape[:-1]:
+        raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} have different leading dims")
+    lead = codes.shape[:-1]
+    flat = [x.reshape(1, 1, -1, x.shape[-1]).contiguous() for x in (codes, scales, biases)]
+    return dequantize_rows(tuple(flat), group_size=group_size, bits=bits)[0].reshape(*lead, -1)
 
 
 FP16_MAX = 65504.0
@@ -890,6 +1090,127 @@ def paged_quantize_append(k: torch.Tensor, k_pool: Triple, v: Optional[torch.Ten
         block_tables.stride(0), st_ptr, int(row_offset), rp, B, H, L, D, int(bits), int(group_size),
         _lib.dtype_code(k.dtype), _lib.stream_ptr(dev))
     _lib.check(rc, "kvq_paged_quantize_append")
+
+
+def _check_starts(starts: Optional[torch.Tensor], B: int, dev) -> Optional[int]:
+    if starts is None:
+        return None
+    if starts.dtype != torch.int32 or tuple(starts.shape) != (B,) or starts.device != dev or not starts.is_contiguous():
+        raise ValueError("starts must be a contiguous int32 tensor of B entries on the same device")
+    return starts.data_ptr()
+
+
+def paged_rope_axes_append(k: torch.Tensor, k_pool: Triple, v: Optional[torch.Tensor], v_pool: Optional[Triple],
+                           block_tables: torch.Tensor, rope: RopeAxes, positions: torch.Tensor, *,
+                           starts: Optional[torch.Tensor] = None, row_offset: int = 0,
+                           queries: Optional[torch.Tensor] = None, group_size: int = 64, bits: int = 8) -> None:
+    """``paged_quantize_append`` with the keys rotated at `positions` (int32 [axes, B, L]) first, and the rows of
+    `queries` [B, Hq, L, D] rotated in place in the same launch."""
+    call = AxesAppendCall(k_pool, v_pool, rope, group_size, bits)
+    rp, B, H, L, D = call._check(k, v, positions, queries)
+    if k_pool[0].shape[1] != H or k_pool[0].shape[2] != PAGE_ROWS:
+        raise ValueError(f"pools must be [num_pages, {H}, {PAGE_ROWS}, *]")
+    _check_table(block_tables, B, call._dev)
+    call._launch(k, v, queries, rp, B, H, L, D, row_offset,
+                 (k_pool[0].shape[0], block_tables.data_ptr(), block_tables.stride(0), _check_starts(starts, B, call._dev)))
+
+
+def paged_dequantize(k_pool: Triple, v_pool: Optional[Triple], block_tables: torch.Tensor, seq_lens: torch.Tensor, *,
+                     group_size: int = 64, bits: int = 8, max_len: Optional[int] = None, out=None):
+    """The first seq_lens[b] rows of every sequence, read back through its block table: (K, V) [B, H, max_len, D]
+    (or (K,) without v_pool). max_len bounds seq_lens (default: out's rows, else the table's capacity). Rows behind
+    a sequence are left as they are in `out`, and are 0 in new tensors."""
+    dev, (_, H, rows), D = _check_read(k_pool, v_pool, group_size, bits)
+    if rows != PAGE_ROWS:
+        raise ValueError(f"pools must be [num_pages, H, {PAGE_ROWS}, *]")
+    B = block_tables.shape[0]
+    _check_table(block_tables, B, dev)
+    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,) or seq_lens.device != dev or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be a contiguous int32 tensor of B entries on the pools' device")
+    if max_len is None:
+        max_len = block_tables.shape[1] * PAGE_ROWS if out is None else tuple(out)[0].shape[2]
+    n = int(max_len)
+    outs = _read_out(out, 1 if v_pool is None else 2, (B, H, n, D), k_pool[1].dtype, dev, torch.zeros)
+    if outs[0].numel() == 0:
+        return outs
+    kq, kr = _lib.qtensor(*k_pool), _lib.rows(outs[0])
+    vq, vr = (None, None) if v_pool is None else (_lib.qtensor(*v_pool), _lib.rows(outs[1]))
+    ref = ctypes.byref
+    with _on_device(dev):
+        rc = _lib.lib().kvq_paged_dequantize(
+            ref(kq), ref(kr), None if vq is None else ref(vq), None if vr is None else ref(vr), k_pool[0].shape[0],
+            block_tables.data_ptr(), block_tables.stride(0), seq_lens.data_ptr(), B, H, n, D, int(bits), int(group_size),
+            _lib.dtype_code(k_pool[1].dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "kvq_paged_dequantize")
+    return outs
+
+
+# ---- keeping accepted rows
+
+def _row_arrays(tensors) -> "ctypes.Array":
+    arr = (_lib.RowArray * len(tensors))()
+    for a, t in zip(arr, tensors):
+        n = t.element_size()
+        a.data, a.row_bytes = t.data_ptr(), t.shape[3] * n
+        a.stride_b, a.stride_h, a.stride_l = (n * s for s in t.stride()[:3])
+    return arr
+
+
+def _check_kept(tensors, rows: torch.Tensor, B: int, n: Optional[int]):
+    if not tensors:
+        raise ValueError("no cache arrays")
+    dev = _require_cuda(*tensors, rows)
+    H = tensors[0].shape[1]
+    for t in tensors:
+        if t.dim() != 4 or t.shape[1] != H or t.stride(3) != 1:
+            raise ValueError(f"cache arrays must be 4-D [*, {H}, rows, width] with contiguous rows, got {tuple(t.shape)}")
+    if rows.dtype != torch.int32 or rows.dim() not in (1, 2) or (rows.dim() == 2 and rows.shape[0] != B) or \
+            (rows.shape[-1] > 1 and rows.stride(-1) != 1):
+        raise ValueError(f"rows must be int32 [B={B}, M] or [M] with contiguous entries, got {rows.dtype} {tuple(rows.shape)}")
+    M = rows.shape[-1]
+    return dev, H, M, (rows.stride(0) if rows.dim() == 2 else 0)
+
+
+def keep_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, start: int, n: int) -> None:
+    """Move the accepted rows of drafted ones up, in place: in every array [B, H, cap, W] of `tensors` (codes, scales,
+    biases, or unquantized rows; any mix of layers), row start + i of sequence b becomes what row start + rows[b, i] held,
+    for the M entries of rows (int32 [B, M] or [M], on the GPU; indices among the n rows from `start`). An entry outside
+    [i, n) leaves its row as it is, so an ascending list padded with -1 keeps fewer rows for some sequences. One launch for
+    up to 192 arrays."""
+    tensors = list(tensors)
+    B = tensors[0].shape[0] if tensors else 0
+    dev, H, M, sb = _check_kept(tensors, rows, B, n)
+    if any(t.shape[0] != B or start < 0 or start + n > t.shape[2] for t in tensors):
+        raise ValueError(f"every array must hold {B} sequences and rows [{start}, {start + n})")
+    if M == 0:
+        return
+    arr = _row_arrays(tensors)
+    with _on_device(dev):
+        rc = _lib.lib().kvq_keep_rows(arr, len(tensors), 0, None, 0, rows.data_ptr(), sb, None, int(start), int(n), M, B, H,
+                                      _lib.stream_ptr(dev))
+    _lib.check(rc, "kvq_keep_rows")
+
+
+def paged_keep_rows(pools: Sequence[Tuple[Triple, Triple]], block_tables: torch.Tensor, rows: torch.Tensor, *,
+                    starts: Optional[torch.Tensor] = None, start: int = 0, n: Optional[int] = None) -> None:
+    """``keep_rows`` over paged pools: `pools` are the layers' (K triple, V triple); sequence b's drafted rows begin at
+    row starts[b] (int32 [B] on the GPU; default: `start` for all). `n`: how many were drafted (default: any row of the
+    table may be named). A row outside the table, or on a page outside the pool, is neither read nor written."""
+    tensors = [t for layer in pools for tr in layer for t in tr]
+    B = block_tables.shape[0]
+    dev, H, M, sb = _check_kept(tensors, rows, B, n)
+    _check_table(block_tables, B, dev)
+    pages = tensors[0].shape[0]
+    if any(t.shape[0] != pages or t.shape[2] != PAGE_ROWS for t in tensors):
+        raise ValueError(f"pools must be [{pages}, H, {PAGE_ROWS}, *]")
+    n = max(M, block_tables.shape[1] * PAGE_ROWS) if n is None else int(n)
+    if M == 0:
+        return
+    arr = _row_arrays(tensors)
+    with _on_device(dev):
+        rc = _lib.lib().kvq_keep_rows(arr, len(tensors), pages, block_tables.data_ptr(), block_tables.stride(0), rows.data_ptr(),
+                                      sb, _check_starts(starts, B, dev), int(start), n, M, B, H, _lib.stream_ptr(dev))
+    _lib.check(rc, "kvq_keep_rows")
 
 
 def paged_attention(queries: torch.Tensor, k_pool: Triple, v_pool: Triple, block_tables: torch.Tensor,

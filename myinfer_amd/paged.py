@@ -176,8 +176,18 @@ class PagedRadixKVCache:
 
     def append(self, layer: int, keys: torch.Tensor, values: torch.Tensor, block_tables: torch.Tensor, *,
                starts: Optional[torch.Tensor] = None, row_offset: int = 0,
-               rope: Optional[kernels.Rope] = None) -> None:
-        """Quantize keys/values [B, Hkv, L, D] into the layer's pages (fused, one launch)."""
+               rope=None, positions: Optional[torch.Tensor] = None, queries: Optional[torch.Tensor] = None) -> None:
+        """Quantize keys/values [B, Hkv, L, D] into the layer's pages (fused, one launch). With a ``kernels.RopeAxes``
+        the keys are rotated at `positions` (int32 [axes, B, L]) first, and `queries` [B, Hq, L, D], if given, in place."""
+        if isinstance(rope, kernels.RopeAxes):
+            if positions is None:
+                raise ValueError("a kernels.RopeAxes needs positions")
+            kernels.paged_rope_axes_append(keys, self._k[layer], values, self._v[layer], block_tables, rope, positions,
+                                           starts=starts, row_offset=row_offset, queries=queries,
+                                           group_size=self.group_size, bits=self.bits)
+            return
+        if positions is not None or queries is not None:
+            raise ValueError("positions and queries go with a kernels.RopeAxes")
         kernels.paged_quantize_append(keys, self._k[layer], values, self._v[layer], block_tables, starts=starts,
                                       row_offset=row_offset, group_size=self.group_size, bits=self.bits, rope=rope)
 
@@ -187,6 +197,18 @@ class PagedRadixKVCache:
         return kernels.paged_attention(queries, self._k[layer], self._v[layer], block_tables, seq_lens, scale,
                                        causal=causal, window=window, group_size=self.group_size, bits=self.bits,
                                        max_len=max_len, kernel=kernel, tree=tree)
+
+    def keep_rows(self, block_tables: torch.Tensor, rows: torch.Tensor, starts: torch.Tensor, n: Optional[int] = None) -> None:
+        """After n drafted rows of every sequence, from row starts[b] on, were verified: row starts[b] + i becomes what
+        row starts[b] + rows[b, i] held (int32 [B, M] ascending, padded with -1), in every layer. The caller's lengths
+        become starts[b] + the rows kept."""
+        kernels.paged_keep_rows(list(zip(self._k, self._v)), block_tables, rows, starts=starts, n=n)
+
+    def dequantized(self, layer: int, block_tables: torch.Tensor, seq_lens: torch.Tensor, max_len: Optional[int] = None,
+                    out=None):
+        """The layer's first seq_lens[b] rows of every sequence read back as values: K and V [B, Hkv, max_len, D]."""
+        return kernels.paged_dequantize(self._k[layer], self._v[layer], block_tables, seq_lens, group_size=self.group_size,
+                                        bits=self.bits, max_len=max_len, out=out)
 
     def gather(self, layer: int, block_table: Sequence[int], length: int):
         """The first `length` rows of one sequence as contiguous [1, Hkv, length, *] triples (K, V)."""
