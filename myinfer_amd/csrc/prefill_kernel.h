@@ -776,7 +776,7 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
     }
   };
   // a tree's 32-key block from k: this lane's keys k + 8 (i / 4) + 4 hh + i % 4
-  auto tree_mask = [&](f16v& acc, int k) {
+  auto tree_mask = [&](f16v& acc, int k) __attribute__((always_inline)) {
     const uint32_t seen = node.keys(k) >> (4 * hh);
     const int lo = lo_r - k - 4 * hh;
 #pragma unroll
