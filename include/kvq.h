@@ -312,10 +312,10 @@ int kvq_draft_tree(const int32_t* parents, int64_t parents_stride_b, int B, int 
  * node's output row is 0.
  *   seq_lens: NULL (S rows each) or device int32 [B], L <= seq_lens[b] <= S: the rows with the tree's.
  *   window:   0 = none; else at least L: keys at positions > the node's position - window only.
- * Calls of many rows run on the prefill kernels (head_dim 64, 96, 128 with output rows 16-byte aligned and, with two
- * or more scale groups a row, 4-byte aligned scale and bias rows; 256), a bf16 cache's only with its range words
- * (kvq_tree_on_prefill says where they are read). Hidden keys' values enter a product with zero: they have to
- * be finite, as under the other masks. workspace: kvq_tree_workspace_size bytes, 256-byte aligned, zero-filled
+ *   scale:    positive.
+ * Calls of some tens of rows a KV head and of more run on kernels of their own, a bf16 cache's only with its range
+ * words (kvq_tree_reads_range says where they are read; without them it runs on the decode kernel). Hidden keys'
+ * values enter a product with zero: they have to be finite, as under the other masks. workspace: kvq_tree_workspace_size bytes, 256-byte aligned, zero-filled
  * when it is allocated.
  */
 int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
@@ -326,7 +326,7 @@ int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v,
 size_t kvq_tree_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window);
 
 /* 1 if kvq_tree_attn may take a kernel that reads a bf16 cache's range words at these sizes, else 0. */
-int kvq_tree_on_prefill(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window);
+int kvq_tree_reads_range(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window);
 
 /* The same over an unquantized cache (kvq_decode_attn_dense's arguments and head dims). */
 int kvq_tree_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,

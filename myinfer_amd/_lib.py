@@ -206,7 +206,7 @@ SIGNATURES = {
     "kvq_tree_attn_dense": (c_int, _DENSE_ARGS[:12] + _TREE_TAIL),
     "kvq_paged_tree_attn": (c_int, _PAGED_ATTN_ARGS[:17] + _TREE_TAIL),
     "kvq_tree_workspace_size": (c_size_t, _WS_ARGS),
-    "kvq_tree_on_prefill": (c_int, [c_int] * 8),
+    "kvq_tree_reads_range": (c_int, [c_int] * 8),
     "kvq_radix_create": (c_void_p, [c_int, c_int]),
     "kvq_radix_destroy": (None, [c_void_p]),
     "kvq_radix_match_and_allocate": (

@@ -736,7 +736,9 @@ int kvq_draft_tree(const int32_t* parents, int64_t parents_stride_b, int B, int 
                     "draft_tree launch");
 }
 
-static int check_tree(const kvq_tree* t, int L, int window) {
+static int check_tree(const kvq_tree* t, int L, float scale, int window) {
+  // (the kernels hide keys before they scale)
+  if (!(scale > 0.0f)) return fail(KVQ_ERR_INVALID, "tree attention needs a positive scale, got %g", (double)scale);
   if (!t || !t->bits || !t->depths) return fail(KVQ_ERR_INVALID, "tree, tree->bits and tree->depths must not be NULL");
   if (!aligned(t->bits, 4) || !aligned(t->depths, 4) || t->bits_stride_b < 0 || t->depths_stride_b < 0)
     return fail(KVQ_ERR_INVALID, "tree bits and depths must be 4-byte aligned with non-negative batch strides");
@@ -746,41 +748,57 @@ static int check_tree(const kvq_tree* t, int L, int window) {
   return KVQ_OK;
 }
 
-// Whether a tree's rows are enough for the prefill kernels (the head_dim-256 one at 256 dims). The decode
-// kernel's time grows with its passes over the keys, a prefill kernel's with its row blocks and the split
-// merge: the line is the one that calls of several passes' rows have measured (kernels._auto_kernel).
-static bool tree_rows_on_prefill(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window, bool dense) {
+// The kernel of a tree call by its sizes. rows: a KV head's query rows; work: the K elements a pass over the cache reads.
+// head_dim 64 and 128: the decode kernel (16 G / D rows a pass) up to 8 rows and where its passes past the third read
+// less than 2^25 elements; the prefill kernel (256 rows a pass) once the rows kernel's blocks of 32 past the fourth
+// read more than 2^25. us, decode / rows / prefill (head_dim 128, groups of 64, 8 KV heads unless said):
+//   20 rows,  4106 keys  11.5 / 13.8 /  22    32 rows, 8 sequences of 4096, 4 bits  32.5 / 26.2 / 53.0
+//   24 rows, 16384 keys  20.1 / 25.8 /  32    64 rows, 8 sequences of 6144, 4 bits  68.9 / 41.7 / 71.8
+//   64 rows,  4096 keys  14.5 / 13.8 /  21   128 rows, 32768 keys                    116 / 48.8 / 53.6
+//   64 rows,  8192 keys  21.6 / 18.7 /  25   192 rows, 32768 keys                    215 / 65.7 / 56.4
+//  256 rows,  2048 keys  20.6 / 20.7 /  24   256 rows, 32768 keys                    215 / 79.9 / 59.6
+//  124 rows of 64 unquantized dims, 4 sequences of 2047: 11.0 / 11.9 / 22
+// head_dim 96 has no rows kernel, head_dim 256 neither: its prefill kernel's lines are kernels._auto_kernel's.
+enum class TreeKernel { kDecode, kRows, kPrefill };
+static TreeKernel tree_kernel_of(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window, bool dense) {
   const int64_t rows = (int64_t)(Hq / Hkv) * L, units = (int64_t)B * Hkv;
-  if (D == 96 && !dense) return rows > 64;
-  if (D != 64 && D != 128 && (D != 256 || dense)) return false;
-  const int per = 16 * group_size / D;
-  if (rows <= std::max(per, 8)) return false;
-  if (dense) return true;
-  const int64_t passes = (rows + per - 1) / per, keys = window > 0 ? std::min(S, window + L) : S;
-  const int64_t block = D == 256 ? 128 : 256, free_passes = D == 256 ? 3 : 4, limit = D == 256 ? 5 << 15 : 330000;
-  return !(rows < block && units * passes <= 512 && (passes - free_passes) * units * keys <= limit);
+  const int64_t keys = window > 0 ? std::min((int64_t)S, (int64_t)window + L) : S;
+  if (D == 96 && !dense) return rows > 64 ? TreeKernel::kPrefill : TreeKernel::kDecode;
+  if ((D != 64 && D != 128 && D != 256) || (D == 256 && dense)) return TreeKernel::kDecode;
+  if (rows <= 8) return TreeKernel::kDecode;
+  const int64_t per = 16 * group_size / D, passes = (rows + per - 1) / per;
+  if (D == 256) {
+    const bool few = rows < 128 && units * passes <= 512 && (passes - 3) * units * keys <= 5 << 15;
+    return few ? TreeKernel::kDecode : TreeKernel::kPrefill;
+  }
+  const int64_t work = units * keys * D, line = 1 << 25;
+  if ((passes - 3) * work < line) return TreeKernel::kDecode;
+  return ((rows + 31) / 32 - 4) * work > line ? TreeKernel::kPrefill : TreeKernel::kRows;
 }
 
-int kvq_tree_on_prefill(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window) {
+int kvq_tree_reads_range(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || S <= 0 || D <= 0 || window < 0 || group_size <= 0 || Hq % Hkv) return 0;
-  return tree_rows_on_prefill(B, Hq, Hkv, L, D, S, group_size, window, false) ? 1 : 0;
+  return tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, false) != TreeKernel::kDecode ? 1 : 0;
 }
 
-// The kernel of a call is chosen by its rows; a call whose tensors the prefill kernels cannot take stays on the
-// decode kernel (unaligned output or scale rows, a bf16 cache without range words).
-static bool tree_on_prefill(const kvq_qtensor* k, const kvq_qtensor* v, const kvq_rows* out, int B, int Hq, int Hkv, int L,
-                            int D, int S, int group_size, int dtype, int window) {
-  if (!tree_rows_on_prefill(B, Hq, Hkv, L, D, S, group_size, window, false)) return false;
-  if (dtype == KVQ_DTYPE_BF16 && (!k->range_exp || !v->range_exp)) return false;
-  if (D == 256) return true;
-  if (!aligned(out->data, 16) || (out->stride_b | out->stride_h | out->stride_l) % 8) return false;
-  return D == 96 || check_prefill_sb(k, v, D, group_size) == KVQ_OK;
+// ... and after: a bf16 cache without range words stays on the decode kernel, whose operands hold any value; a call whose
+// output or scale rows the prefill kernel cannot take runs on the rows kernel, which can.
+static TreeKernel tree_kernel_for(const kvq_qtensor* k, const kvq_qtensor* v, const kvq_rows* out, int B, int Hq, int Hkv,
+                                  int L, int D, int S, int group_size, int dtype, int window) {
+  const TreeKernel t = tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, k == nullptr);
+  if (t == TreeKernel::kDecode) return t;
+  if (k && dtype == KVQ_DTYPE_BF16 && (!k->range_exp || !v->range_exp)) return TreeKernel::kDecode;
+  if (t == TreeKernel::kRows || D == 256) return t;
+  const bool rows16 = aligned(out->data, 16) && !((out->stride_b | out->stride_h | out->stride_l) % 8);
+  const bool ok = (rows16 || (!k && D == 64)) && (!k || D == 96 || check_prefill_sb(k, v, D, group_size) == KVQ_OK);
+  return ok ? t : D == 96 ? TreeKernel::kDecode : TreeKernel::kRows;
 }
 
 size_t kvq_tree_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window) {
   size_t n = kvq_decode_workspace_size(B, Hq, Hkv, L, D, S, window);
   if (n == 0 || Hq % Hkv) return 0;
   if (D == 64 || D == 96 || D == 128) n = std::max(n, kvq::prefill_tree_bytes(B, Hq, Hkv, L, D, S, window));
+  if (D == 64 || D == 128) n = std::max(n, kvq::tree_rows_bytes(B, Hq, Hkv, L, D, S, window));
   return n;  // (the decode size covers the head_dim-256 kernel)
 }
 
@@ -790,11 +808,12 @@ int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v,
   if (check_head_dim(D, "tree attention")) return KVQ_ERR_UNSUPPORTED;
   int rc = check_attn(q, k, v, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, window,
                       kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window), workspace, workspace_bytes);
-  if (rc || (rc = check_tree(tree, L, window))) return rc;
+  if (rc || (rc = check_tree(tree, L, scale, window))) return rc;
+  const TreeKernel kernel = tree_kernel_for(k, v, out, B, Hq, Hkv, L, D, S, group_size, dtype, window);
   hipError_t e;
-  if (!tree_on_prefill(k, v, out, B, Hq, Hkv, L, D, S, group_size, dtype, window)) {
+  if (kernel != TreeKernel::kPrefill) {
     e = kvq::launch_decode(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, 0, window, workspace,
-                           (hipStream_t)stream, nullptr, tree);
+                           (hipStream_t)stream, nullptr, tree, kernel == TreeKernel::kRows);
   } else if (D == 256) {
     e = kvq::launch_wide(q, k, v, seq_lens, out, B, Hq, Hkv, L, S, bits, group_size, dtype, scale, 0, window, workspace,
                          (hipStream_t)stream, tree);
@@ -813,12 +832,14 @@ int kvq_paged_tree_attn(const kvq_rows* q, const kvq_qtensor* k_pool, const kvq_
   int rc = check_paged_attn(q, k_pool, v_pool, num_pages, block_table, table_stride, out, B, Hq, Hkv, L, D, S, bits,
                             group_size, dtype, scale, window, kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window),
                             workspace, workspace_bytes);
-  if (rc || (rc = check_tree(tree, L, window))) return rc;
+  if (rc || (rc = check_tree(tree, L, scale, window))) return rc;
   if (!seq_lens) return fail(KVQ_ERR_INVALID, "seq_lens is NULL");
+  const TreeKernel kernel = tree_kernel_for(k_pool, v_pool, out, B, Hq, Hkv, L, D, S, group_size, dtype, window);
   hipError_t e;
-  if (!tree_on_prefill(k_pool, v_pool, out, B, Hq, Hkv, L, D, S, group_size, dtype, window)) {
+  if (kernel != TreeKernel::kPrefill) {
     e = kvq::launch_decode_paged(q, k_pool, v_pool, num_pages, block_table, table_stride, seq_lens, out, B, Hq, Hkv, L, D, S,
-                                 bits, group_size, dtype, scale, 0, window, workspace, (hipStream_t)stream, tree);
+                                 bits, group_size, dtype, scale, 0, window, workspace, (hipStream_t)stream, tree,
+                                 kernel == TreeKernel::kRows);
   } else if (D == 256) {
     e = kvq::launch_wide_paged(q, k_pool, v_pool, num_pages, block_table, table_stride, seq_lens, out, B, Hq, Hkv, L, S, bits,
                                group_size, dtype, scale, 0, window, workspace, (hipStream_t)stream, tree);
@@ -835,18 +856,18 @@ int kvq_tree_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v,
   if (check_head_dim(D, "unquantized tree attention")) return KVQ_ERR_UNSUPPORTED;
   int rc = check_attn_dense(q, k, v, out, B, Hq, Hkv, L, D, S, dtype, scale, window,
                             kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window), workspace, workspace_bytes);
-  if (rc || (rc = check_tree(tree, L, window))) return rc;
-  const bool rows16 = aligned(out->data, 16) && !((out->stride_b | out->stride_h | out->stride_l) % 8);
+  if (rc || (rc = check_tree(tree, L, scale, window))) return rc;
+  const TreeKernel kernel = tree_kernel_for(nullptr, nullptr, out, B, Hq, Hkv, L, D, S, 64, dtype, window);
   hipError_t e;
   if (D > 128) {  // unquantized rows past 128 dims run through the head_dim-256 kernel
     e = kvq::launch_wide_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,
                                (hipStream_t)stream, nullptr, tree);
-  } else if (tree_rows_on_prefill(B, Hq, Hkv, L, D, S, 64, window, true) && (D == 64 || rows16)) {
+  } else if (kernel == TreeKernel::kPrefill) {
     e = kvq::launch_prefill_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,
                                   (hipStream_t)stream, tree);
   } else {
     e = kvq::launch_decode_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,
-                                 (hipStream_t)stream, nullptr, tree);
+                                 (hipStream_t)stream, nullptr, tree, kernel == TreeKernel::kRows);
   }
   return hip_status(e, "tree_attn_dense launch");
 }

@@ -213,7 +213,7 @@ static void set_mask(DecParams& p, const kvq_mask* mask) {
 hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                          const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,
                          float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask,
-                         const kvq_tree* tree) {
+                         const kvq_tree* tree, bool tree_rows) {
   const int Dk = decode_kernel_dim(D);
   const DecPlan pl = decode_plan(B, Hq, Hkv, L, Dk, S, window, bits, G);
   DecParams p = decode_params(q, seq_lens, out, Hq, Hkv, L, Dk, S, scale, causal, window, workspace, pl);
@@ -239,6 +239,9 @@ hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qten
   p.vsb_ss = v->sb_stride_s;
   if (tree) {
     p.tree = tree_params(tree, L);
+    p.k_rexp = k->range_exp;
+    p.v_rexp = v->range_exp;
+    if (tree_rows) return launch_tree_rows(p, B, dtype, D, bits, G, false, workspace, stream);
     return launch_decode_tree(p, dtype, Dk, bits, G, false, stream);
   }
   if (!mask && D == Dk && multi_rows(p.nrows, pl.R)) return launch_decode_multi(p, dtype, Dk, bits, G, false, stream);
@@ -250,7 +253,7 @@ hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qten
 hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                                const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                                int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype, float scale,
-                               int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
+                               int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree, bool tree_rows) {
   const int Dk = decode_kernel_dim(D);
   const DecPlan pl = decode_plan(B, Hq, Hkv, L, Dk, S, window, bits, G);
   DecParams p = decode_params(q, seq_lens, out, Hq, Hkv, L, Dk, S, scale, causal, window, workspace, pl);
@@ -278,6 +281,9 @@ hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kv
   p.num_pages = num_pages;
   if (tree) {
     p.tree = tree_params(tree, L);
+    p.k_rexp = k->range_exp;
+    p.v_rexp = v->range_exp;
+    if (tree_rows) return launch_tree_rows(p, B, dtype, D, bits, G, true, workspace, stream);
     return launch_decode_tree(p, dtype, Dk, bits, G, true, stream);
   }
   if (D == Dk && multi_rows(p.nrows, pl.R)) return launch_decode_multi(p, dtype, Dk, bits, G, true, stream);
@@ -289,7 +295,7 @@ hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kv
 hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                                const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
                                int causal, int window, void* workspace, hipStream_t stream, const kvq_mask* mask,
-                               const kvq_tree* tree) {
+                               const kvq_tree* tree, bool tree_rows) {
   const int Dk = decode_kernel_dim(D);
   const DecPlan pl = decode_plan(B, Hq, Hkv, L, Dk, S, window, 16, 64);
   DecParams p = decode_params(q, seq_lens, out, Hq, Hkv, L, Dk, S, scale, causal, window, workspace, pl);
@@ -307,6 +313,7 @@ hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_r
   if (Dk == 256) return hipErrorInvalidValue;  // unquantized rows past 128 dims run through the head_dim-256 kernel
   if (tree) {
     p.tree = tree_params(tree, L);
+    if (tree_rows) return launch_tree_rows(p, B, dtype, D, 16, 64, false, workspace, stream);
     return launch_decode_tree(p, dtype, Dk, 16, 64, false, stream);
   }
   if (Dk == 128) return bf ? launch_decode_shape<BF16, 128, 16>(p, pl, stream) : launch_decode_shape<F16, 128, 16>(p, pl, stream);

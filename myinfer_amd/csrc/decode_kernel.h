@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "dma.h"
 #include "launch.h"
 #include "merge.h"
 #include "tree.h"
@@ -126,6 +127,10 @@ struct DecParams {
   Div31 d_nsplit, d_rowblocks, d_hkv, d_l;
   // a tree of drafted tokens (TREE kernels): the last L rows of a sequence are its nodes
   TreeParams tree;
+  // the caches' range exponents (kvq_qtensor.range_exp), or null: read by tree_attn_kernel, whose operands are
+  // staged times 2^-E; the decode kernel applies scales in fp32 and reads none
+  const int32_t* k_rexp;
+  const int32_t* v_rexp;
 };
 
 // A general mask (kvq_mask) on the lane's 8 scores of a tile (keys k0 + 16 (s / 4) + 4 lg + s % 4 of
@@ -166,11 +171,6 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint8_t* lds, ui
 }
 __device__ __forceinline__ void dma2(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t vo, uint32_t so) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 2, vo, so, 0, 0);
-}
-
-// 32-bit LDS address of a pointer into shared memory.
-__device__ __forceinline__ uint32_t lds_addr(const void* p) {
-  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
 // The LDS operands of one 32-key tile, read by one asm block that also waits for them. The reads
@@ -1212,6 +1212,9 @@ constexpr bool narrow_rows() {
 
 // decode_tree.hip: the TREE launches (p.tree set), any number of rows; bits 16: unquantized caches.
 hipError_t launch_decode_tree(const DecParams& p, int dtype, int D, int bits, int G, bool paged, hipStream_t stream);
+
+// tree_attn.hip: tree_attn_kernel's launches over the operands of `p` (its plan is set there); bits 16: unquantized.
+hipError_t launch_tree_rows(DecParams p, int B, int dtype, int D, int bits, int G, bool paged, void* workspace, hipStream_t stream);
 
 // decode_multi.hip: the MULTI launches, over contiguous caches and paged pools.
 hipError_t launch_decode_multi(const DecParams& p, int dtype, int D, int bits, int G, bool paged, hipStream_t stream);

@@ -25,22 +25,24 @@ hipError_t launch_rope(const kvq_rows* x, const kvq_rope_params* rope, int B, in
 // of the output are stored.
 int decode_kernel_dim(int D);
 size_t decode_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window, int bits, int G);
-// mask: a general mask (kvq_mask) or nullptr; tree: a tree of drafted tokens (kvq_tree) or nullptr
+// mask: a general mask (kvq_mask) or nullptr; tree: a tree of drafted tokens (kvq_tree) or nullptr,
+// tree_rows: on the kernel for some tens of rows (tree_attn.hip; head_dim 64 and 128), whose workspace tree_rows_bytes gives
 hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                          const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,
                          float scale, int causal, int window, void* workspace, hipStream_t stream,
-                         const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr);
+                         const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr, bool tree_rows = false);
 
 hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, int num_pages,
                                const int32_t* table, int64_t table_stride, const int32_t* seq_lens, const kvq_rows* out,
                                int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype, float scale,
                                int causal, int window, void* workspace, hipStream_t stream,
-                               const kvq_tree* tree = nullptr);
+                               const kvq_tree* tree = nullptr, bool tree_rows = false);
 hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,
                                const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype, float scale,
                                int causal, int window, void* workspace, hipStream_t stream,
-                               const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr);
+                               const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr, bool tree_rows = false);
 
+size_t tree_rows_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
 size_t prefill_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
 hipError_t launch_prefill(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                           const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,

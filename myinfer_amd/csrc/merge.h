@@ -140,8 +140,8 @@ inline hipError_t launch_combine(const MergeParams& m, int B, hipStream_t stream
   mm.d_l = make_div31((uint32_t)m.L);
   mm.d_hq = make_div31((uint32_t)m.Hq);
   mm.d_rep = make_div31((uint32_t)m.rep);
-  // R (rows per unit: 16 / scale groups per row for decode, 128 for the head_dim-256 kernel) fixes
-  // the kernel's split strides
+  // R (rows per unit: 16 / scale groups per row for decode, 32 for the tree rows kernel, 128 for the head_dim-256
+  // kernel) fixes the kernel's split strides
   if (dv != D) {
     switch (m.R) {
       case 4: hipLaunchKernelGGL((combine_kernel<T, D, 4, true>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
@@ -156,6 +156,7 @@ inline hipError_t launch_combine(const MergeParams& m, int B, hipStream_t stream
     case 4: hipLaunchKernelGGL((combine_kernel<T, D, 4>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 8: hipLaunchKernelGGL((combine_kernel<T, D, 8>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 16: hipLaunchKernelGGL((combine_kernel<T, D, 16>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
+    case 32: hipLaunchKernelGGL((combine_kernel<T, D, 32>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 128: hipLaunchKernelGGL((combine_kernel<T, D, 128>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     default: return hipErrorInvalidValue;
   }

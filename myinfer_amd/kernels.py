@@ -835,7 +835,7 @@ def _tree_sizes(*sizes: int) -> Tuple[int, int]:
     B, Hq, Hkv, L, D, S, group_size, window = sizes
     lib = _lib.lib()
     return (lib.kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window),
-            lib.kvq_tree_on_prefill(B, Hq, Hkv, L, D, S, group_size, window))
+            lib.kvq_tree_reads_range(B, Hq, Hkv, L, D, S, group_size, window))
 
 
 def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq_lens, group_size, bits, causal, kernel,
@@ -845,7 +845,7 @@ def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq
     dev = queries.device
     Hkv, S = keys.shape[1:3] if dense else keys[0].shape[1:3]
     _check_tree_call(tree, B, L, S, window, causal, kernel, dev)
-    nbytes, prefill = _tree_sizes(B, Hq, Hkv, L, D, S, 64 if dense else group_size, int(window))
+    nbytes, ranges = _tree_sizes(B, Hq, Hkv, L, D, S, 64 if dense else group_size, int(window))
     if nbytes == 0:
         raise NotImplementedError(f"tree attention does not support B={B} Hq={Hq} Hkv={Hkv} L={L} D={D} S={S}")
     stream = _lib.stream_ptr(dev)
@@ -857,7 +857,7 @@ def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq
         symbol, kq, vq, form = "kvq_tree_attn_dense", _lib.rows(keys), _lib.rows(values), ()
     else:
         # a bf16 cache's range words, as prepare_attention has them
-        if prefill and queries.dtype == torch.bfloat16:
+        if ranges and queries.dtype == torch.bfloat16:
             kw, vw = range_word(keys[0]), range_word(values[0])
             if one_shot:
                 kw = range_exponent(keys, bits) if kw is None else kw
@@ -889,7 +889,7 @@ def layer_attention(queries: torch.Tensor, keys, values, scale: float, *, causal
     prefill = _auto_kernel(Hq // Hkv * L, D, group_size, dense=False, units=B * Hkv,
                            keys=min(S, window + L) if window else S) == "prefill"
     kw = vw = None
-    if prefill and queries.dtype == torch.bfloat16:  # the range words, which only these kernels read
+    if ranges and queries.dtype == torch.bfloat16:  # the range words, which only these kernels read
         kw, vw = range_word(keys[0]), range_word(values[0])
         if kw is None or vw is None:
             return None

@@ -83,7 +83,7 @@ QUANT = [
     (1, 16, 8, 128, 64, 8, torch.float16, 10, 4106, "random", 0),
     (2, 8, 2, 128, 64, 8, torch.bfloat16, 33, 33, "gaps", 0),       # no prefix
     (2, 32, 4, 128, 64, 4, torch.float16, 16, 1000, "random", 0),
-    (1, 64, 8, 128, 64, 8, torch.bfloat16, 64, 2111, "gaps", 0),    # prefill kernel
+    (1, 64, 8, 128, 64, 8, torch.bfloat16, 64, 2111, "gaps", 0),    # rows kernel
     (1, 8, 1, 128, 128, 4, torch.bfloat16, 130, 777, "random", 0),
     (1, 32, 4, 128, 32, 8, torch.float16, 31, 513, "random", 0),
     (1, 16, 2, 64, 64, 8, torch.bfloat16, 65, 900, "random", 0),

@@ -92,6 +92,8 @@ def _call(form="quant", **kw):
     (dict(D=100), _lib.ERR_UNSUPPORTED, "multiples of 8"),
     (dict(Hq=7, Hkv=2), _lib.ERR_INVALID, "multiple"),
     (dict(scale=float("nan")), _lib.ERR_INVALID, "scale"),
+    (dict(scale=0.0), _lib.ERR_INVALID, "positive scale"),
+    (dict(scale=-0.1), _lib.ERR_INVALID, "positive scale"),
     (dict(ws=None), _lib.ERR_WORKSPACE, "workspace"),
     (dict(ws=WS + 64), _lib.ERR_WORKSPACE, "aligned"),
     (dict(out=_fake_rows(ptr=(1 << 23) + 2)), _lib.ERR_INVALID, "out"),
@@ -122,8 +124,8 @@ def test_tree_workspace_covers_both_kernels():
     assert lib.kvq_tree_workspace_size(2, 30, 8, 4, 128, 5000, 0) == 0
     assert lib.kvq_tree_workspace_size(2, 32, 8, 0, 128, 5000, 0) == 0
     # few rows stay on the decode kernel, which reads no range words
-    assert lib.kvq_tree_on_prefill(1, 8, 8, 8, 128, 5000, 64, 0) == 0
-    assert lib.kvq_tree_on_prefill(1, 64, 8, 64, 128, 32768, 64, 0) == 1
+    assert lib.kvq_tree_reads_range(1, 8, 8, 8, 128, 5000, 64, 0) == 0
+    assert lib.kvq_tree_reads_range(1, 64, 8, 64, 128, 32768, 64, 0) == 1
 
 
 def test_draft_tree_refuses():
