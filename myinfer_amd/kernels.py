@@ -889,7 +889,7 @@ def layer_attention(queries: torch.Tensor, keys, values, scale: float, *, causal
     prefill = _auto_kernel(Hq // Hkv * L, D, group_size, dense=False, units=B * Hkv,
                            keys=min(S, window + L) if window else S) == "prefill"
     kw = vw = None
-    if ranges and queries.dtype == torch.bfloat16:  # the range words, which only these kernels read
+    if prefill and queries.dtype == torch.bfloat16:  # the range words, which only these kernels read
         kw, vw = range_word(keys[0]), range_word(values[0])
         if kw is None or vw is None:
             return None
