@@ -332,6 +332,11 @@ def bind_host(module, *addresses: int) -> None:
     module.bind(*addresses, ABI_VERSION, ctypes.sizeof(AppendState), torch.__version__)
 
 
+# The entry points of a drafted step, in the order the native host path takes them.
+DRAFT_SYMBOLS = ("kvq_draft_tree", "kvq_tree_attn", "kvq_tree_attn_dense", "kvq_paged_tree_attn", "kvq_tree_workspace_size",
+                 "kvq_tree_reads_range", "kvq_rope_axes", "kvq_rope_axes_append", "kvq_dequantize", "kvq_paged_dequantize",
+                 "kvq_keep_rows")
+
 _host = None
 
 
@@ -354,5 +359,6 @@ def host():
                 bind_host(_kvqhost, *(ctypes.cast(fn, c_void_p).value for fn in (
                     handle.kvq_decode_attn, handle.kvq_prefill_attn, handle.kvq_decode_workspace_size,
                     handle.kvq_prefill_workspace_size)))
+                _kvqhost.bind_draft(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in DRAFT_SYMBOLS))
                 _host = _kvqhost
     return _host

@@ -365,6 +365,9 @@ class QuantizedKVCache:
         stop = self.offset if stop is None else stop
         if self.keys is None or not 0 <= start <= stop <= self.offset:
             raise ValueError(f"rows [{start}, {stop}) of a cache of {self.offset}")
+        both = kernels.read_rows(self.keys, self.values, start, stop, group_size=self.group_size, bits=self.bits)
+        if both is not None:
+            return both
         return kernels.dequantize_rows(tuple(x[:, :, start:stop] for x in self.keys),
                                        tuple(x[:, :, start:stop] for x in self.values), group_size=self.group_size,
                                        bits=self.bits)
@@ -445,17 +448,18 @@ def keep_rows(cache: List, start: int, rows: torch.Tensor) -> int:
     if not torch.is_tensor(rows):
         raise ValueError("rows must be an int32 tensor on the caches' device")
     end = cache[0].offset
-    tensors = []
+    arrays = []
     for c in cache:
         if type(c) not in (KVCache, QuantizedKVCache):
             raise ValueError(f"rows of a {type(c).__name__} are not kept by index")
         if c.keys is None or c.offset != end:
             raise ValueError("the caches must hold rows, all at one offset")
-        tensors += [c.keys, c.values] if type(c) is KVCache else [*c.keys, *c.values]
+        arrays += (c.keys, c.values)
     M = rows.shape[-1] if rows.dim() else 0
     if not 0 <= start <= end or M > end - start:
         raise ValueError(f"{M} rows cannot be kept of rows [{start}, {end})")
-    kernels.keep_rows(tensors, rows, start, end - start)
+    if not kernels.move_rows(arrays, rows, start, end - start):
+        kernels.keep_rows([x for a in arrays for x in ((a,) if torch.is_tensor(a) else a)], rows, start, end - start)
     for c in cache:
         c.offset = start + M
     return start + M

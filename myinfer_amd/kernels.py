@@ -55,6 +55,15 @@ def _on_device(dev: torch.device):
     return torch.cuda.device(dev)
 
 
+def _native(t) -> tuple:
+    """(the native host path, the raw current stream) for a tensor on the current GPU, else (None, 0). What its functions
+    answer: the result, None (the Python path serves or refuses the call), or a failed launch's status."""
+    dev = t.get_device() if torch.is_tensor(t) else -1
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        return None, 0
+    return _lib.host(), torch._C._cuda_getCurrentRawStream(dev)
+
+
 def _check_triple(tr: Sequence[torch.Tensor], name: str) -> None:
     if len(tr) != 3:
         raise ValueError(f"{name} must be a (codes, scales, biases) triple")
@@ -194,9 +203,20 @@ def _set_positions(desc: "_lib.Axes", positions: torch.Tensor, B: int, L: int, d
     desc.positions, desc.pos_stride_a, desc.pos_stride_b, desc.pos_stride_l = positions.data_ptr(), sa, sb, sl
 
 
+_axes_desc = functools.lru_cache(maxsize=64)(RopeAxes.params)
+
+
 def rope_axes(x: torch.Tensor, r: RopeAxes, positions: torch.Tensor) -> torch.Tensor:
     """Rotate x [B, H, L, D] (float16/bfloat16, CUDA) in place, row l of sequence b at positions[:, b, l], and return
     it. positions: int32 [axes, B, L] or [axes, L]."""
+    host, stream = _native(x)
+    if host is not None:
+        desc = _axes_desc(r)
+        done = host.rope_axes(ctypes.addressof(desc), x, positions, stream)
+        if done is True:
+            return x
+        if done is not None:
+            _lib.check(done, "kvq_rope_axes")
     dev = _require_cuda(x)
     if x.dim() != 4:
         raise ValueError(f"x must be [B, H, L, D], got {tuple(x.shape)}")
@@ -236,6 +256,11 @@ class AxesAppendCall:
         self._dtype, self._code = scales.dtype, _lib.dtype_code(scales.dtype)
         self._bits, self._group = int(bits), int(group_size)
         self._rp = rope.params()
+        self._state = _lib.AppendState(
+            None, ctypes.addressof(self._kq), None if self._vq is None else ctypes.addressof(self._vq),
+            ctypes.addressof(self._rp), *self._lead, self._rows, *self._widths, self._bits, self._group, self._code,
+            self._dev.index, None)
+        self._state_ptr = ctypes.addressof(self._state)
 
     def _check(self, k, v, positions, queries) -> tuple:
         if k.dtype != self._dtype or k.device != self._dev or k.dim() != 4:
@@ -271,6 +296,13 @@ class AxesAppendCall:
 
     def __call__(self, k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, row_offset: int,
                  queries: Optional[torch.Tensor] = None) -> None:
+        host, stream = _native(k)
+        if host is not None:
+            done = host.axes_append(self._state_ptr, k, v, positions, row_offset, queries, stream)
+            if done is True:
+                return
+            if done is not None:
+                _lib.check(done, "kvq_rope_axes_append")
         rp, B, H, L, D = self._check(k, v, positions, queries)
         if (B, H) != self._lead:
             raise ValueError(f"destination leads {self._lead} do not match source {(B, H)}")
@@ -468,9 +500,26 @@ def _read_out(out, n: int, shape, dtype, dev, fresh):
     return out
 
 
+def read_rows(k: Triple, v: Triple, start: int, stop: int, *, group_size: int = 64, bits: int = 8, out=None, table=None,
+              seq_lens=None):
+    """Rows [start, stop) of K and V triples through the native host path, as ``dequantize_rows`` of those rows or, with a
+    block table, ``paged_dequantize`` into `out`; None for a call it does not take."""
+    host, stream = _native(k[1])
+    if host is None:
+        return None
+    got = host.dequantize(k, v, start, stop, group_size, bits, out, table, seq_lens, stream)
+    if type(got) is int:
+        _lib.check(got, "kvq_dequantize" if table is None else "kvq_paged_dequantize")
+    return got
+
+
 def dequantize_rows(k: Triple, v: Optional[Triple] = None, *, group_size: int = 64, bits: int = 8, out=None):
     """The rows of quantized triples [B, H, S, *] (views of a cache) as values [B, H, S, D] in their dtype, K and V in
     one launch: (K, V), or (K,) without v. `out`: the tensors to fill instead of new ones."""
+    if v is not None and type(k) is tuple and len(k) == 3 and k[0].dim() == 4:
+        got = read_rows(k, v, 0, k[0].shape[2], group_size=group_size, bits=bits, out=None if out is None else tuple(out))
+        if got is not None:
+            return got
     dev, (B, H, S), D = _check_read(k, v, group_size, bits)
     outs = _read_out(out, 1 if v is None else 2, (B, H, S, D), k[1].dtype, dev, torch.empty)
     if outs[0].numel() == 0:
@@ -586,44 +635,68 @@ class DraftTree:
     refilled in place (and into a graph)."""
 
     def __init__(self, parents: torch.Tensor, starts=None):
-        dev = _require_cuda(parents)
-        if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or parents.shape[-1] < 1:
-            raise ValueError(f"parents must be int32 [B, L] or [L] with L >= 1, got {parents.dtype} {tuple(parents.shape)}")
-        L = parents.shape[-1]
-        if L > _lib.TREE_MAX_NODES:
-            raise NotImplementedError(f"a tree has at most {_lib.TREE_MAX_NODES} nodes, got {L}")
-        if parents.stride(-1) != 1 and L > 1:
-            raise ValueError("the nodes of parents must be contiguous")
+        self._starts = starts
+        host, stream = _native(parents)
+        buf = None if host is None else host.draft_tree(parents, starts, stream)
+        if type(buf) is int:
+            _lib.check(buf, "kvq_draft_tree")
+        if buf is None:  # checked, served or refused here
+            dev = _require_cuda(parents)
+            if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or parents.shape[-1] < 1:
+                raise ValueError(f"parents must be int32 [B, L] or [L] with L >= 1, got {parents.dtype} {tuple(parents.shape)}")
+            L = parents.shape[-1]
+            if L > _lib.TREE_MAX_NODES:
+                raise NotImplementedError(f"a tree has at most {_lib.TREE_MAX_NODES} nodes, got {L}")
+            if parents.stride(-1) != 1 and L > 1:
+                raise ValueError("the nodes of parents must be contiguous")
+            B = 1 if parents.dim() == 1 else parents.shape[0]
+            if torch.is_tensor(starts):
+                if starts.dtype != torch.int32 or starts.device != dev or tuple(starts.shape) != (B,) or \
+                        not starts.is_contiguous():
+                    raise ValueError(f"starts must be an int or a contiguous int32 tensor of {B} entries on {dev}")
+            elif starts is not None:
+                self._starts = int(starts)
+                if not -2 ** 31 <= self._starts < 2 ** 31 - L:
+                    raise ValueError(f"start {starts} leaves the int32 positions")
         self.parents = parents
+        self.device = parents.device
         self.shared = parents.dim() == 1  # one tree for any batch
-        self.B, self.L = (1 if self.shared else parents.shape[0]), L
-        self._starts, self._start = None, 0
-        if torch.is_tensor(starts):
-            if starts.dtype != torch.int32 or starts.device != dev or tuple(starts.shape) != (self.B,) or \
-                    not starts.is_contiguous():
-                raise ValueError(f"starts must be an int or a contiguous int32 tensor of {self.B} entries on {dev}")
-            self._starts = starts
-        elif starts is not None:
-            self._start = int(starts)
-            if not -2 ** 31 <= self._start < 2 ** 31 - L:
-                raise ValueError(f"start {self._start} leaves the int32 positions")
-        words = (L + 31) // 32
-        n = self.B * L
-        buf = torch.empty(n * (words + (2 if starts is not None else 1)), dtype=torch.int32, device=dev)
-        self.bits = buf[: n * words].view(self.B, L, words)
-        self.depths = buf[n * words: n * (words + 1)].view(self.B, L)
-        self.positions = None if starts is None else buf[n * (words + 1):].view(1, self.B, L)
-        self.desc = _lib.Tree(self.bits.data_ptr(), self.depths.data_ptr(), 0 if self.shared else L * words,
-                              0 if self.shared else L)
-        self.device = dev
-        self.refresh()
+        self.B, self.L = (1 if self.shared else parents.shape[0]), parents.shape[-1]
+        self._words, self._nodes = (self.L + 31) // 32, self.B * self.L
+        self._buf = buf
+        if buf is None:
+            self._buf = torch.empty(self._nodes * (self._words + (1 if starts is None else 2)), dtype=torch.int32,
+                                    device=self.device)
+            self.refresh()
+
+    @functools.cached_property
+    def bits(self) -> torch.Tensor:
+        return self._buf[: self._nodes * self._words].view(self.B, self.L, self._words)
+
+    @functools.cached_property
+    def depths(self) -> torch.Tensor:
+        n = self._nodes * self._words
+        return self._buf[n: n + self._nodes].view(self.B, self.L)
+
+    @functools.cached_property
+    def positions(self) -> Optional[torch.Tensor]:
+        n = self._nodes * (self._words + 1)
+        return None if self._starts is None else self._buf[n:].view(1, self.B, self.L)
+
+    @functools.cached_property
+    def desc(self) -> "_lib.Tree":
+        at = self._buf.data_ptr()
+        return _lib.Tree(at, at + 4 * self._nodes * self._words, 0 if self.shared else self.L * self._words,
+                         0 if self.shared else self.L)
 
     def refresh(self) -> None:
+        tensor = torch.is_tensor(self._starts)
         with _on_device(self.device):
             rc = _lib.lib().kvq_draft_tree(
-                self.parents.data_ptr(), 0 if self.shared else self.parents.stride(0), self.B, self.L, self.bits.data_ptr(),
-                self.depths.data_ptr(), None if self._starts is None else self._starts.data_ptr(), self._start,
-                None if self.positions is None else self.positions.data_ptr(), _lib.stream_ptr(self.device))
+                self.parents.data_ptr(), 0 if self.shared else self.parents.stride(0), self.B, self.L, self.desc.bits,
+                self.desc.depths, self._starts.data_ptr() if tensor else None,
+                0 if tensor or self._starts is None else self._starts,
+                None if self._starts is None else self.positions.data_ptr(), _lib.stream_ptr(self.device))
         _lib.check(rc, "kvq_draft_tree")
 
     def check(self, B: int, L: int, device) -> None:
@@ -871,6 +944,24 @@ def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq
     return _DeviceCall(dev, getattr(_lib.lib(), symbol), args, keep, "tree", out, symbol)
 
 
+def _tree_attention(queries, keys, values, scale, tree: DraftTree, window, seq_lens, group_size, bits, table=None,
+                    max_len=None) -> Optional[torch.Tensor]:
+    """Attention over a tree through the native host path (`keys` and `values` are pools with a block table); None for a
+    call it does not take, and under capture, where the call has a workspace of its own."""
+    host, stream = _native(queries)
+    if host is None or type(window) is not int or torch.cuda.is_current_stream_capturing():
+        return None
+    dev = queries.get_device()
+    head = (queries, keys, values, scale, window, seq_lens, group_size, bits, _range_words)
+    tail = (stream, tree._buf, 0 if tree.shared else tree.B, tree.L, table, -1 if max_len is None else max_len)
+    out = host.tree_attention(*head, _workspaces.get((dev, stream)), *tail)
+    if type(out) is int and out > 0:  # the bytes of workspace it needs
+        out = host.tree_attention(*head, _workspace(queries.device, stream, out), *tail)
+    if type(out) is int:  # a failed launch, which is not tried again
+        _lib.check(out, "kvq_tree_attn" if table is None else "kvq_paged_tree_attn")
+    return out
+
+
 def layer_attention(queries: torch.Tensor, keys, values, scale: float, *, causal: bool, window: int = 0,
                     seq_lens: Optional[torch.Tensor] = None, group_size: int = 64,
                     bits: int = 8) -> Optional[torch.Tensor]:
@@ -918,7 +1009,11 @@ def attention(queries: torch.Tensor, keys, values, scale: float, *, causal: bool
     that where its passes over the keys cost less than the prefill kernel's row blocks).
 
     With `tree` the queries are the nodes of a DraftTree, whose keys are each sequence's last L rows (of
-    seq_lens[b] >= L, or of S); a window must then be at least L."""
+    seq_lens[b] >= L, or of S); a window must then be at least L, and the scale positive."""
+    if tree is not None and out is None and kernel == "auto" and not causal:
+        got = _tree_attention(queries, keys, values, scale, tree, window, seq_lens, group_size, bits)
+        if got is not None:
+            return got
     return prepare_attention(queries, keys, values, scale, causal=causal, window=window, seq_lens=seq_lens,
                              group_size=group_size, bits=bits, out=out, kernel=kernel, tree=tree, _one_shot=True)()
 
@@ -1120,6 +1215,12 @@ def paged_dequantize(k_pool: Triple, v_pool: Optional[Triple], block_tables: tor
     """The first seq_lens[b] rows of every sequence, read back through its block table: (K, V) [B, H, max_len, D]
     (or (K,) without v_pool). max_len bounds seq_lens (default: out's rows, else the table's capacity). Rows behind
     a sequence are left as they are in `out`, and are 0 in new tensors."""
+    if out is not None and v_pool is not None and type(k_pool) is tuple and len(out) == 2:
+        out = tuple(out)
+        got = read_rows(k_pool, v_pool, 0, out[0].shape[2] if max_len is None else int(max_len), group_size=group_size,
+                        bits=bits, out=out, table=block_tables, seq_lens=seq_lens)
+        if got is not None:
+            return got
     dev, (_, H, rows), D = _check_read(k_pool, v_pool, group_size, bits)
     if rows != PAGE_ROWS:
         raise ValueError(f"pools must be [num_pages, H, {PAGE_ROWS}, *]")
@@ -1171,6 +1272,16 @@ def _check_kept(tensors, rows: torch.Tensor, B: int, n: Optional[int]):
     return dev, H, M, (rows.stride(0) if rows.dim() == 2 else 0)
 
 
+def move_rows(tensors, rows, start: int, n: int, table=None, starts=None) -> bool:
+    """``keep_rows``, or with a block table ``paged_keep_rows``, through the native host path, of tensors in nested lists and
+    tuples; False for a call it does not take."""
+    host, stream = _native(rows)
+    done = None if host is None else host.keep_rows(tensors, rows, start, n, table, starts, stream)
+    if done is not None and done is not True:
+        _lib.check(done, "kvq_keep_rows")
+    return done is True
+
+
 def keep_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, start: int, n: int) -> None:
     """Move the accepted rows of drafted ones up, in place: in every array [B, H, cap, W] of `tensors` (codes, scales,
     biases, or unquantized rows; any mix of layers), row start + i of sequence b becomes what row start + rows[b, i] held,
@@ -1178,6 +1289,8 @@ def keep_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, start: int, n
     [i, n) leaves its row as it is, so an ascending list padded with -1 keeps fewer rows for some sequences. One launch for
     up to 192 arrays."""
     tensors = list(tensors)
+    if move_rows(tensors, rows, start, n):
+        return
     B = tensors[0].shape[0] if tensors else 0
     dev, H, M, sb = _check_kept(tensors, rows, B, n)
     if any(t.shape[0] != B or start < 0 or start + n > t.shape[2] for t in tensors):
@@ -1196,6 +1309,10 @@ def paged_keep_rows(pools: Sequence[Tuple[Triple, Triple]], block_tables: torch.
     """``keep_rows`` over paged pools: `pools` are the layers' (K triple, V triple); sequence b's drafted rows begin at
     row starts[b] (int32 [B] on the GPU; default: `start` for all). `n`: how many were drafted (default: any row of the
     table may be named). A row outside the table, or on a page outside the pool, is neither read nor written."""
+    if n is None and torch.is_tensor(block_tables) and block_tables.dim() == 2 and torch.is_tensor(rows) and rows.dim():
+        n = max(rows.shape[-1], block_tables.shape[1] * PAGE_ROWS)
+    if n is not None and move_rows(pools, rows, start, n, block_tables, starts):
+        return
     tensors = [t for layer in pools for tr in layer for t in tr]
     B = block_tables.shape[0]
     dev, H, M, sb = _check_kept(tensors, rows, B, n)
@@ -1222,6 +1339,10 @@ def paged_attention(queries: torch.Tensor, k_pool: Triple, v_pool: Triple, block
     pages block_tables[b]; queries [B, Hq, L, D] sit at its last L positions (or are the nodes of `tree`,
     which those rows hold; `workspace` is then the caller's, if given). max_len bounds seq_lens (default: the
     table's capacity) and sizes the split plan."""
+    if tree is not None and out is None and kernel == "auto" and not causal and workspace is None:
+        got = _tree_attention(queries, k_pool, v_pool, scale, tree, window, seq_lens, group_size, bits, block_tables, max_len)
+        if got is not None:
+            return got
     _check_triple(k_pool, "k_pool")
     _check_triple(v_pool, "v_pool")
     dev = _require_cuda(queries, *k_pool, *v_pool)
