@@ -313,9 +313,9 @@ int kvq_draft_tree(const int32_t* parents, int64_t parents_stride_b, int B, int 
  *   seq_lens: NULL (S rows each) or device int32 [B], L <= seq_lens[b] <= S: the rows with the tree's.
  *   window:   0 = none; else at least L: keys at positions > the node's position - window only.
  *   scale:    positive.
- * Calls of some tens of rows a KV head and of more run on kernels of their own, a bf16 cache's only with its range
- * words (kvq_tree_reads_range says where they are read; without them it runs on the decode kernel). Hidden keys'
- * values enter a product with zero: they have to be finite, as under the other masks. workspace: kvq_tree_workspace_size bytes, 256-byte aligned, zero-filled
+ * Calls of some tens of rows a KV head and of more run on kernels of their own; those of the most rows read a bf16
+ * cache's range words (kvq_tree_reads_range says where), and without them run slower. Hidden keys' values enter a
+ * product with zero: they have to be finite, as under the other masks. workspace: kvq_tree_workspace_size bytes, 256-byte aligned, zero-filled
  * when it is allocated.
  */
 int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,

@@ -778,20 +778,21 @@ static TreeKernel tree_kernel_of(int B, int Hq, int Hkv, int L, int D, int S, in
 
 int kvq_tree_reads_range(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || S <= 0 || D <= 0 || window < 0 || group_size <= 0 || Hq % Hkv) return 0;
-  return tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, false) != TreeKernel::kDecode ? 1 : 0;
+  return tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, false) == TreeKernel::kPrefill ? 1 : 0;
 }
 
-// ... and after: a bf16 cache without range words stays on the decode kernel, whose operands hold any value; a call whose
-// output or scale rows the prefill kernel cannot take runs on the rows kernel, which can.
+// ... and after: what the prefill kernel cannot take (a bf16 cache without range words, output or scale rows that are not
+// aligned for it) runs on the rows kernel, of a width that has none on the decode kernel.
 static TreeKernel tree_kernel_for(const kvq_qtensor* k, const kvq_qtensor* v, const kvq_rows* out, int B, int Hq, int Hkv,
                                   int L, int D, int S, int group_size, int dtype, int window) {
   const TreeKernel t = tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, k == nullptr);
-  if (t == TreeKernel::kDecode) return t;
-  if (k && dtype == KVQ_DTYPE_BF16 && (!k->range_exp || !v->range_exp)) return TreeKernel::kDecode;
-  if (t == TreeKernel::kRows || D == 256) return t;
-  const bool rows16 = aligned(out->data, 16) && !((out->stride_b | out->stride_h | out->stride_l) % 8);
-  const bool ok = (rows16 || (!k && D == 64)) && (!k || D == 96 || check_prefill_sb(k, v, D, group_size) == KVQ_OK);
-  return ok ? t : D == 96 ? TreeKernel::kDecode : TreeKernel::kRows;
+  if (t != TreeKernel::kPrefill) return t;
+  bool ok = !k || dtype != KVQ_DTYPE_BF16 || (k->range_exp && v->range_exp);
+  if (D != 256) {
+    const bool rows16 = aligned(out->data, 16) && !((out->stride_b | out->stride_h | out->stride_l) % 8);
+    ok = ok && (rows16 || (!k && D == 64)) && (!k || D == 96 || check_prefill_sb(k, v, D, group_size) == KVQ_OK);
+  }
+  return ok ? t : D == 64 || D == 128 ? TreeKernel::kRows : TreeKernel::kDecode;
 }
 
 size_t kvq_tree_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window) {

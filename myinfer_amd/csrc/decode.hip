@@ -239,8 +239,6 @@ hipError_t launch_decode(const kvq_rows* q, const kvq_qtensor* k, const kvq_qten
   p.vsb_ss = v->sb_stride_s;
   if (tree) {
     p.tree = tree_params(tree, L);
-    p.k_rexp = k->range_exp;
-    p.v_rexp = v->range_exp;
     if (tree_rows) return launch_tree_rows(p, B, dtype, D, bits, G, false, workspace, stream);
     return launch_decode_tree(p, dtype, Dk, bits, G, false, stream);
   }
@@ -281,8 +279,6 @@ hipError_t launch_decode_paged(const kvq_rows* q, const kvq_qtensor* k, const kv
   p.num_pages = num_pages;
   if (tree) {
     p.tree = tree_params(tree, L);
-    p.k_rexp = k->range_exp;
-    p.v_rexp = v->range_exp;
     if (tree_rows) return launch_tree_rows(p, B, dtype, D, bits, G, true, workspace, stream);
     return launch_decode_tree(p, dtype, Dk, bits, G, true, stream);
   }

@@ -127,10 +127,6 @@ struct DecParams {
   Div31 d_nsplit, d_rowblocks, d_hkv, d_l;
   // a tree of drafted tokens (TREE kernels): the last L rows of a sequence are its nodes
   TreeParams tree;
-  // the caches' range exponents (kvq_qtensor.range_exp), or null: read by tree_attn_kernel, whose operands are
-  // staged times 2^-E; the decode kernel applies scales in fp32 and reads none
-  const int32_t* k_rexp;
-  const int32_t* v_rexp;
 };
 
 // A general mask (kvq_mask) on the lane's 8 scores of a tile (keys k0 + 16 (s / 4) + 4 lg + s % 4 of

@@ -17,8 +17,9 @@
 //    their scales and biases, which the wave's lanes converted once per tile into a small table.
 //  * Splits are merged as the decode kernel's are: up to 4 by the last to finish, more by combine_kernel.
 // Operands and roundings are the prefill kernel's: q times a power of two in fp16 (exact), K and V dequantized to fp16
-// (times 2^-E, the cache's range exponent), probabilities in fp16, everything else in fp32; an unquantized cache
-// runs in its own type.
+// (a bf16 cache's times 2^-E), probabilities in fp16, everything else in fp32; an unquantized cache runs in its own
+// type. E follows from the scales and biases of the tile itself (K) or of the wave's tiles so far (V), 0 while they fit
+// fp16: the cache's range word is not needed, so pages without one do not have to fall back on the decode kernel.
 //
 // Measured with the merge (decode kernel / here / prefill kernel, us): 8 KV heads over 32768 keys of 128 dims in 8 bits
 // (75 MB, 14.5 us as a copy), 32 rows 38.7 / 31.3 / 51.0, 64 rows 64.5 / 32.7 / 50.8, 128 rows 116 / 48.8 / 53.6;
@@ -110,6 +111,29 @@ template <typename T>
 __device__ __forceinline__ _Float16 operand_half(uint32_t cell, float m) {
   if constexpr (T::id == KVQ_DTYPE_BF16) return (_Float16)(__uint_as_float(cell << 16) * m);
   return __builtin_bit_cast(_Float16, (uint16_t)cell);
+}
+
+// The larger of |bias| and |bias + top code * scale|: what a group's values are bounded by.
+template <int BITS>
+__device__ __forceinline__ float group_bound(uint32_t s_cell, uint32_t b_cell) {
+  const float s = __uint_as_float(s_cell << 16), b = __uint_as_float(b_cell << 16);
+  return fmaxf(fabsf(b), fabsf(fmaf((float)((1 << BITS) - 1), s, b)));
+}
+
+constexpr float kHalfSafe = 32768.0f;  // operands stay within it (the rounding of a value next to 65504 may not)
+
+// The smallest e >= 0 with every lane's bound <= 2^15 2^e (bounds that are NaN ask for nothing).
+__device__ __forceinline__ int bound_exponent(float bound) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) bound = fmaxf(bound, __shfl_xor(bound, m));
+  int e = 0;
+  if (bound > kHalfSafe) {
+    const float f = frexpf(bound * (1.0f / kHalfSafe), &e);  // bound <= 2^15 2^e
+    if (f == 0.5f) --e;
+    e = min(max(e, 0), 127);
+    if (bound == INFINITY) e = 127;
+  }
+  return e;
 }
 
 // Keys of a workgroup: the sequence's keys from `base` in whole tiles, an even share for each split that is a multiple of
@@ -241,17 +265,9 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
     for (int j = 0; j < C::SLOTS; ++j) issue(j);
   }
 
-  // ---- range exponents (bf16 caches), query operand
-  float kmul = 1.0f, vmul = 1.0f, vback = 1.0f, inv2 = p.scale_log2;
+  // ---- query operand
+  float inv2 = p.scale_log2;
   if constexpr (!C::DENSE) {
-    int ek = 0;
-    if constexpr (T::id == KVQ_DTYPE_BF16) {
-      const int ev = p.v_rexp ? min(max(*p.v_rexp, 0), 127) : 0;
-      ek = p.k_rexp ? min(max(*p.k_rexp, 0), 127) : 0;
-      kmul = ldexpf(1.0f, -ek);
-      vmul = ldexpf(1.0f, -ev);
-      vback = ldexpf(1.0f, ev);
-    }
     float qmax = 0.0f;
 #pragma unroll
     for (int j = 0; j < C::KSTEPS; ++j)
@@ -264,7 +280,7 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
     if (qmax > 0.0f) frexpf(qmax, &e);
     const int qe = 14 - e;  // |q| 2^qe < 2^14, exact
     const float qmul = ldexpf(1.0f, qe);
-    inv2 = ldexpf(inv2, ek - qe);
+    inv2 = ldexpf(inv2, -qe);
 #pragma unroll
     for (int j = 0; j < C::KSTEPS; ++j)
 #pragma unroll
@@ -275,6 +291,9 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
 
   const int lo_all = p.window > 0 ? max(0, S_b - p.window) : 0;
   float m_run = -INFINITY, l_run = 0.0f;
+  constexpr bool kRange = !C::DENSE && T::id == KVQ_DTYPE_BF16;  // values may leave the fp16 range
+  int ev = 0;                   // V's exponent so far (uniform)
+  float vmul = 1.0f, vback = 1.0f, vlimit = kHalfSafe;  // 2^-ev, 2^ev, 2^15 2^ev
   f16v oacc[C::DPL];
 #pragma unroll
   for (int db = 0; db < C::DPL; ++db) oacc[db] = f16v{};
@@ -293,12 +312,40 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
     asm volatile("s_waitcnt vmcnt(%0)" ::"i"((C::SLOTS - 1) * C::IPT) : "memory");  // tile i has landed
     // ---- the tile's operands into registers
     uint32_t kcell[2][KG] = {};
+    float kmul = 1.0f, inv2t = inv2;
     if constexpr (!C::DENSE) {
       const uint32_t* cells = (const uint32_t*)(sl + 2 * C::TB);
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
         kcell[0][g] = cells[32 * (kg0 + g) + n];
         kcell[1][g] = cells[C::AS / 4 + 32 * (kg0 + g) + n];
+      }
+      if constexpr (kRange) {
+        float kb = 0.0f, vb = 0.0f;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) kb = fmaxf(kb, group_bound<BITS>(kcell[0][g], kcell[1][g]));
+#pragma unroll
+        for (int h = 0; h < C::NSB; ++h) {
+          const int c = 64 * h + (C::NG >= 2 ? 32 * hh : 0) + n;
+          vb = fmaxf(vb, group_bound<BITS>(cells[2 * C::AS / 4 + c], cells[3 * C::AS / 4 + c]));
+        }
+        if (__builtin_amdgcn_ballot_w64(kb > kHalfSafe) != 0) {
+          const int ek = bound_exponent(kb);
+          kmul = ldexpf(1.0f, -ek);
+          inv2t = ldexpf(inv2, ek);
+        }
+        if (__builtin_amdgcn_ballot_w64(vb > vlimit) != 0) {
+          const int e = max(bound_exponent(vb), ev);
+          const float f = ldexpf(1.0f, ev - e);
+#pragma unroll
+          for (int db = 0; db < C::DPL; ++db)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) oacc[db][x] *= f;
+          ev = e;
+          vmul = ldexpf(1.0f, -ev);
+          vback = ldexpf(1.0f, ev);
+          vlimit = ldexpf(kHalfSafe, min(ev, 112));  // (past it every finite bound is within)
+        }
       }
       // V's, converted once: lane -> group 2 h + hh of key n
 #pragma unroll
@@ -415,7 +462,7 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
     float tm = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) tm = fmaxf(tm, s[e]);
-    tm = max_xor32(tm) * inv2;
+    tm = max_xor32(tm) * inv2t;
     if (__builtin_amdgcn_ballot_w64(tm > m_run + kSlack) != 0) {
       const float m_new = tm > m_run + kSlack ? fmaxf(m_run, tm) : m_run;
       const float corr = m_new == m_run ? 1.0f : exp2_fast(m_run - m_new);
@@ -432,8 +479,8 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const float p0 = exp2_fast(fmaf(s[8 * t + 2 * a], inv2, nm));
-        const float p1 = exp2_fast(fmaf(s[8 * t + 2 * a + 1], inv2, nm));
+        const float p0 = exp2_fast(fmaf(s[8 * t + 2 * a], inv2t, nm));
+        const float p1 = exp2_fast(fmaf(s[8 * t + 2 * a + 1], inv2t, nm));
         pop[t][a] = pack2(p0, p1, OT{});
         l_run = add_pair(pop[t][a], l_run, OT{});
       }
@@ -460,9 +507,9 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
     for (int e = 0; e < 16; ++e) {
       float* dst = w_o + at * C::ORow + C::DPL * (8 * (e >> 2) + 4 * hh + (e & 3));
       if constexpr (C::DPL == 4) {
-        *(f4*)dst = f4{oacc[0][e], oacc[1][e], oacc[2][e], oacc[3][e]};
+        *(f4*)dst = f4{oacc[0][e] * vback, oacc[1][e] * vback, oacc[2][e] * vback, oacc[3][e] * vback};
       } else {
-        *(float2*)dst = make_float2(oacc[0][e], oacc[1][e]);
+        *(float2*)dst = make_float2(oacc[0][e] * vback, oacc[1][e] * vback);
       }
     }
   }
@@ -501,7 +548,6 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
         l += f * w_l[w * C::R + rr];
       }
     }
-    o *= vback;  // (V's operands were scaled by 2^-E)
     if (single) {
       uint16_t* dst = out_row(rr);
       if (dst) write_out(dst + d0, o, l > 0.0f ? 1.0f / l : 0.0f);

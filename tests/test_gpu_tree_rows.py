@@ -49,7 +49,7 @@ CASES = [
 def test_quantized(B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window):
     print(f"tree rows B={B} Hq={Hq} Hkv={Hkv} D={D} G={G} bits={bits} {dtype} L={L} S={S} {kind} window={window}", flush=True)
     assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window)
-    assert _lib.lib().kvq_tree_reads_range(B, Hq, Hkv, L, D, S, G, window) == 1
+    assert _lib.lib().kvq_tree_reads_range(B, Hq, Hkv, L, D, S, G, window) == 0  # (which only the prefill kernel does)
     kt, vt = make_cache(B, Hkv, S, D, bits, dtype, 340 + L, group=G)
     q = seeded_normal((B, Hq, L, D), 341 + S, dtype, DEV)
     parents = make_parents(kind, B, L, 342 + D)
@@ -178,8 +178,8 @@ def test_views_and_unaligned_outputs(pad, off):
 
 
 def test_bf16_cache_with_and_without_range_words():
-    """A bf16 cache beyond the fp16 range: with its range words on the rows kernel, through pages without them on the
-    decode kernel, whose operands hold it."""
+    """A bf16 cache beyond the fp16 range: the rows kernel finds its operands' exponents itself, with or without range
+    words, from the tiles' scales and biases."""
     from tests.test_gpu_paged import build
 
     Hq, Hkv, D, L, lens = 64, 8, 128, 20, [1000, 333]
@@ -215,6 +215,40 @@ def test_nonfinite_values_stay_hidden():
     out = kernels.attention(q, k, v, 0.1, tree=kernels.DraftTree(tensor(parents)))
     assert_close(out[:, :, :-1], ref[:, :, :-1], "others")
     assert not out[:, :, 2].any() and not torch.isfinite(out[:, :, -1]).any()
+
+
+@pytest.mark.parametrize("G,bits,D", [(64, 8, 128), (32, 4, 128), (128, 8, 128), (32, 8, 64), (64, 4, 64)])
+def test_bf16_ranges_by_tile(G, bits, D):
+    """K and V rows of a bf16 cache whose magnitudes grow and shrink by powers of two from tile to tile, up to 2^40 (K
+    2^20): every power of two is exact. With V's, queries of zero weigh all keys alike; with K's, queries of 2^-19 keep the
+    scores of the usual size, so that the operands' rounding moves them as little as in the other tests."""
+    Hq, Hkv, L, S, B = 64, 8, 30, 3000 if 16 * G // D > 8 else 1500, 2
+    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S)
+    kt, vt = make_cache(B, Hkv, S, D, bits, torch.bfloat16, 420, group=G)
+    p2 = torch.ones(S, dtype=torch.float32)
+    for at, n, e in [(64, 40, 20), (333, 5, 40), (700, 1, 17), (1201, 64, 33)]:
+        p2[at:at + n] = 2.0 ** e
+    p2 = p2.to(DEV)[None, None, :, None]
+    big = [tuple([c, (s.float() * m).bfloat16(), (b.float() * m).bfloat16()]) for (c, s, b), m in ((kt, p2), (vt, p2))]
+    q = torch.zeros(B, Hq, L, D, dtype=torch.bfloat16, device=DEV)  # no weight depends on the large keys
+    parents = make_parents("random", B, L, 421)
+    tree = kernels.DraftTree(tensor(parents))
+    out = kernels.attention(q, big[0], big[1], 0.1, group_size=G, bits=bits, tree=tree)
+    top = 2.0 ** 40
+    ref = exact(q, values_of(big[0], torch.bfloat16, G, bits) / top, values_of(big[1], torch.bfloat16, G, bits) / top, 0.1, parents,
+                [S] * B, S)
+    scale = abs(ref).max()
+    assert_close((out.float() / (top * scale)).bfloat16(), ref / scale, "V by tile")
+    # large keys, queries so small that the scores are of the usual size
+    p2 = torch.ones(S, dtype=torch.float32)
+    for at, n, e in [(64, 40, 20), (333, 5, 18), (700, 1, 17), (1201, 64, 19)]:
+        p2[at:at + n] = 2.0 ** e
+    p2 = p2.to(DEV)[None, None, :, None]
+    kbig = (kt[0], (kt[1].float() * p2).bfloat16(), (kt[2].float() * p2).bfloat16())
+    q = seeded_normal((B, Hq, L, D), 422, torch.bfloat16, DEV) * 2.0 ** -19
+    out = kernels.attention(q, kbig, vt, 0.1, group_size=G, bits=bits, tree=tree)
+    ref = exact(q, values_of(kbig, torch.bfloat16, G, bits), values_of(vt, torch.bfloat16, G, bits), 0.1, parents, [S] * B, S)
+    assert_close(out, ref, "K by tile")
 
 
 @pytest.mark.parametrize("amp", [0.0, 1e-4, 60.0])
