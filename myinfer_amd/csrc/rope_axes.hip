@@ -8,9 +8,13 @@
 // the angle, 2e-3 rad at position 32768, twice what rounding the result to fp16 costs. The rotation
 // is in fp32, its products rounded before they are added, as in kvq_rope; the result is rounded to T.
 //
-// What bounds it: each row is read and written once (rotated in place, or read and stored quantized), and a
-// pair's sine and cosine cost more than its rotation. A workgroup therefore takes some positions of
-// several heads: it forms the sines and cosines of its positions once, into LDS, and every head's rows use them.
+// What bounds it: each row is read and written once (rotated in place, or read and stored quantized), and a pair's
+// sine and cosine cost more than its rotation, so heads share them: in a thread's registers where rows are rotated in
+// place, in a table in LDS where a workgroup quantizes some positions of several heads.
+//
+// Rotated in place (4096 tokens of 32 heads of 128 dims, 67 MB): 12.1 us with 4 heads a thread, 5.5 TB/s, the rate of a
+// large copy; 13.3 with 2, 17.6 with 1, and 29.1 with the table, whose barrier each row waited for. At 1024 tokens
+// 6.9 / 6.2 / 6.9 us with 4 / 2 / 1, at 16 tokens of 64 heads 5.9 / 4.7 / 5.8 (a launch takes 3.6).
 
 #include "quantize_core.h"
 
@@ -22,10 +26,10 @@ constexpr int kTableCells = 2048;  // (position, pair) cells of a workgroup's ta
 struct AxesArgs {
   const int32_t* pos;
   int64_t pos_sa, pos_sb, pos_sl;
-  int dims, pairs, traditional;
+  int dims, pairs, traditional, axes;
   Div31 div_pairs;
   double freq[kAxesPairs];  // times the position scale
-  uint8_t axis[kAxesPairs];
+  alignas(8) uint8_t axis[kAxesPairs];
 };
 
 // sin and cos of an angle in radians: k pi/2 + t, |t| <= pi/4 (off by k 2^-54, nothing up to 2^31), and the
@@ -82,91 +86,86 @@ __device__ __forceinline__ Rows rows_of(const RowCut& c, int wg, int L, int H) {
 struct RotateJob {
   uint16_t* x;
   int64_t s_b, s_h, s_l;
-  int H;
-  RowCut cut;
-  Div31 div_items;  // items (8 pairs each) of a row
+  int H, L, per_row, groups, heads;  // items (8 pairs each) of a row, groups of `heads` heads
+  uint32_t items;                    // threads: a position's 8 pairs of a group of heads each
+  Div31 div_row, div_l, div_groups;
+  int blocks;
 };
 
-// Rotate rows in place: a thread takes 8 pairs of a row at a time (split halves: dims [8j, +8) and [8j + dims/2,
-// +8); interleaved: dims [16j, +16)), the next item's loads issued before the present one is computed.
-template <typename T>
-__device__ __forceinline__ void rotate_rows(const RotateJob& job, const AxesArgs& r, const Rows& rows, float2* tab) {
+// Rotate rows in place. A thread takes 8 pairs of a position (split halves: dims [8j, +8) and [8j + dims/2, +8);
+// interleaved: dims [16j, +16)) in NH heads, whose rows it loads first; their sines and cosines stay in its registers.
+template <typename T, int NH>
+__device__ __forceinline__ void rotate_rows(const RotateJob& job, const AxesArgs& r, uint32_t wg) {
 #pragma clang fp contract(off)
-  const int per_row = r.pairs / 8, items = rows.nh * rows.nl * per_row;
+  const uint32_t t = wg * 256 + threadIdx.x;
+  if (t >= job.items) return;
+  const uint32_t row = div31(t, job.div_row), j = t - row * job.per_row;
+  const uint32_t bg = div31(row, job.div_l), l = row - bg * job.L;
+  const uint32_t b = div31(bg, job.div_groups);
+  const int h0 = (int)(bg - b * job.groups) * NH, nh = min(NH, job.H - h0);
   const int second = r.traditional ? 8 : r.dims / 2;
-  const uint32_t nl = (uint32_t)rows.nl;
-  auto at = [&](int i, int& l, int& j) -> uint16_t* {
-    const int row = (int)div31((uint32_t)i, job.div_items);
-    j = i - row * per_row;
-    const int h = (int)((uint32_t)row / nl);
-    l = row - h * rows.nl;
-    return job.x + (int64_t)rows.b * job.s_b + (int64_t)(rows.h0 + h) * job.s_h + (int64_t)(rows.l0 + l) * job.s_l +
-           (r.traditional ? 16 : 8) * j;
-  };
-  int i = threadIdx.x, l = 0, j = 0;
-  uint16_t* p = nullptr;
-  u4 lo{}, hi{};
-  if (i < items) {
-    p = at(i, l, j);
-    lo = *(const u4*)p;
-    hi = *(const u4*)(p + second);
+  uint16_t* const x = job.x + (int64_t)b * job.s_b + (int64_t)h0 * job.s_h + (int64_t)l * job.s_l + (r.traditional ? 16 : 8) * j;
+  u4 lo[NH], hi[NH];
+#pragma unroll
+  for (int k = 0; k < NH; ++k) {
+    const uint16_t* p = x + (int64_t)min(k, nh - 1) * job.s_h;
+    lo[k] = *(const u4*)p;
+    hi[k] = *(const u4*)(p + second);
   }
-  fill_table(r, rows.b, rows.l0, rows.nl, tab);
-  __syncthreads();
-  while (i < items) {
-    const int ni = i + 256;
-    uint16_t* np = nullptr;
-    int n_l = 0, nj = 0;
-    u4 nlo{}, nhi{};
-    if (ni < items) {
-      np = at(ni, n_l, nj);
-      nlo = *(const u4*)np;
-      nhi = *(const u4*)(np + second);
+  float2 cs[8];
+  {
+    const int32_t* at = r.pos + (int64_t)b * r.pos_sb + (int64_t)l * r.pos_sl;
+    int32_t pos[KVQ_MAX_AXES];
+#pragma unroll
+    for (int a = 0; a < KVQ_MAX_AXES; ++a) pos[a] = at[(int64_t)min(a, r.axes - 1) * r.pos_sa];
+    const u2 axes = *(const u2*)(r.axis + 8 * j);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t a = (axes[e / 4] >> (8 * (e % 4))) & 0xffu;
+      const int32_t q = a < 2 ? (a == 0 ? pos[0] : pos[1]) : (a == 2 ? pos[2] : pos[3]);
+      cs[e] = cos_sin((double)q * r.freq[8 * j + e]);
     }
+  }
+#pragma unroll
+  for (int k = 0; k < NH; ++k) {
     float a[16];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      a[2 * e] = to_float((uint16_t)(lo[e] & 0xffffu), T{});
-      a[2 * e + 1] = to_float((uint16_t)(lo[e] >> 16), T{});
-      a[8 + 2 * e] = to_float((uint16_t)(hi[e] & 0xffffu), T{});
-      a[8 + 2 * e + 1] = to_float((uint16_t)(hi[e] >> 16), T{});
+      a[2 * e] = to_float((uint16_t)(lo[k][e] & 0xffffu), T{});
+      a[2 * e + 1] = to_float((uint16_t)(lo[k][e] >> 16), T{});
+      a[8 + 2 * e] = to_float((uint16_t)(hi[k][e] & 0xffffu), T{});
+      a[8 + 2 * e + 1] = to_float((uint16_t)(hi[k][e] >> 16), T{});
     }
-    const float2* cs = tab + l * r.pairs + 8 * j;
     uint16_t o[16];
+    auto turn = [&](int x0, int y0, int e) {
+      const float u = a[x0] * cs[e].x - a[y0] * cs[e].y, v = a[x0] * cs[e].y + a[y0] * cs[e].x;
+      o[x0] = from_float(u, T{});
+      o[y0] = from_float(v, T{});
+    };
+    if (r.traditional) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 t = cs[e];
-      const float x = r.traditional ? a[2 * e] : a[e], y = r.traditional ? a[2 * e + 1] : a[8 + e];
-      const uint16_t u = from_float(x * t.x - y * t.y, T{}), v = from_float(x * t.y + y * t.x, T{});
-      if (r.traditional) {
-        o[2 * e] = u;
-        o[2 * e + 1] = v;
-      } else {
-        o[e] = u;
-        o[8 + e] = v;
+      for (int e = 0; e < 8; ++e) turn(2 * e, 2 * e + 1, e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) turn(e, 8 + e, e);
+    }
+    if (k < nh) {
+      uint16_t* p = x + (int64_t)k * job.s_h;
+      u4 wl, wh;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        wl[e] = (uint32_t)o[2 * e] | ((uint32_t)o[2 * e + 1] << 16);
+        wh[e] = (uint32_t)o[8 + 2 * e] | ((uint32_t)o[8 + 2 * e + 1] << 16);
       }
+      *(u4*)p = wl;
+      *(u4*)(p + second) = wh;
     }
-    u4 wl, wh;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      wl[e] = (uint32_t)o[2 * e] | ((uint32_t)o[2 * e + 1] << 16);
-      wh[e] = (uint32_t)o[8 + 2 * e] | ((uint32_t)o[8 + 2 * e + 1] << 16);
-    }
-    *(u4*)p = wl;
-    *(u4*)(p + second) = wh;
-    i = ni;
-    p = np;
-    l = n_l;
-    j = nj;
-    lo = nlo;
-    hi = nhi;
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void rope_axes_kernel(RotateJob job, AxesArgs r, int L) {
-  __shared__ float2 tab[kTableCells];
-  rotate_rows<T>(job, r, rows_of(job.cut, (int)blockIdx.x, L, job.H), tab);
+template <typename T, int NH>
+__global__ __launch_bounds__(256) void rope_axes_kernel(RotateJob job, AxesArgs r) {
+  rotate_rows<T, NH>(job, r, blockIdx.x);
 }
 
 struct AppendJob {
@@ -271,7 +270,10 @@ __global__ __launch_bounds__(256) void rope_axes_append_kernel(AppendJob a, Rota
     }
     wg -= a.cut.blocks;
   }
-  rotate_rows<T>(q, r, rows_of(q.cut, wg, a.L, q.H), tab);
+  if (q.heads == 2)
+    rotate_rows<T, 2>(q, r, (uint32_t)wg);
+  else
+    rotate_rows<T, 4>(q, r, (uint32_t)wg);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -286,6 +288,7 @@ static AxesArgs make_axes(const kvq_axes* p) {
   r.dims = p->dims;
   r.pairs = p->dims / 2;
   r.traditional = p->traditional;
+  r.axes = p->axes;
   r.div_pairs = make_div31((uint32_t)r.pairs);
   int left[KVQ_MAX_AXES], count[KVQ_MAX_AXES] = {};
   for (int a = 0; a < p->axes; ++a) left[a] = p->sections[a];
@@ -321,6 +324,8 @@ static RowCut cut_rows(int B, int H, int L, int per_row, int pairs) {
   return c;
 }
 
+constexpr int64_t kManyItems = 1 << 19;  // a head's 8 pairs; 4 heads a thread from here on (2048 tokens of 32 heads)
+
 static RotateJob make_rotate(const kvq_rows* x, int B, int H, int L, int pairs) {
   RotateJob j{};
   j.x = (uint16_t*)x->data;
@@ -328,20 +333,35 @@ static RotateJob make_rotate(const kvq_rows* x, int B, int H, int L, int pairs) 
   j.s_h = x->stride_h;
   j.s_l = x->stride_l;
   j.H = H;
-  j.cut = cut_rows(B, H, L, pairs / 8, pairs);
-  j.div_items = make_div31((uint32_t)(pairs / 8));
+  j.L = L;
+  j.per_row = pairs / 8;
+  const int64_t one = (int64_t)B * L * j.per_row;
+  j.heads = one * H >= kManyItems ? 4 : 2;
+  j.groups = (H + j.heads - 1) / j.heads;
+  const int64_t items = one * j.groups;
+  if (items >= (int64_t)1 << 31) return j;
+  j.items = (uint32_t)items;
+  j.blocks = (int)((items + 255) / 256);
+  j.div_row = make_div31((uint32_t)j.per_row);
+  j.div_l = make_div31((uint32_t)L);
+  j.div_groups = make_div31((uint32_t)j.groups);
   return j;
 }
 
 hipError_t launch_rope_axes(const kvq_rows* x, const kvq_axes* rope, int B, int H, int L, int dtype, hipStream_t stream) {
   const AxesArgs r = make_axes(rope);
   const RotateJob j = make_rotate(x, B, H, L, r.pairs);
-  if (!j.cut.blocks) return hipErrorInvalidValue;
-  if (dtype == KVQ_DTYPE_BF16)
-    hipLaunchKernelGGL((rope_axes_kernel<BF16>), dim3(j.cut.blocks), dim3(256), 0, stream, j, r, L);
-  else
-    hipLaunchKernelGGL((rope_axes_kernel<F16>), dim3(j.cut.blocks), dim3(256), 0, stream, j, r, L);
-  return hipGetLastError();
+  if (!j.blocks) return hipErrorInvalidValue;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const dim3 grid(j.blocks), block(256);
+    if (j.heads == 2)
+      hipLaunchKernelGGL((rope_axes_kernel<T, 2>), grid, block, 0, stream, j, r);
+    else
+      hipLaunchKernelGGL((rope_axes_kernel<T, 4>), grid, block, 0, stream, j, r);
+    return hipGetLastError();
+  };
+  return dtype == KVQ_DTYPE_BF16 ? go(BF16{}) : go(F16{});
 }
 
 template <typename T, int BITS, int G>
@@ -352,7 +372,7 @@ static hipError_t launch_append(AppendJob a, const RotateJob& q, const AxesArgs&
   a.div_chunks = make_div31((uint32_t)a.per_row);
   a.cut = cut_rows(B, a.H, a.L, a.per_row, r.pairs);
   if (!a.cut.blocks) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(a.cut.blocks * (1 + a.values) + q.cut.blocks));
+  const dim3 grid((unsigned)(a.cut.blocks * (1 + a.values) + q.blocks));
   if (wide)
     hipLaunchKernelGGL((rope_axes_append_kernel<T, BITS, G, 32>), grid, dim3(256), 0, stream, a, q, r);
   else
@@ -378,7 +398,7 @@ hipError_t launch_rope_axes_append(const kvq_rows* k_src, const kvq_qtensor* k_d
   RotateJob qj{};
   if (q) {
     qj = make_rotate(q, B, Hq, L, r.pairs);
-    if (!qj.cut.blocks) return hipErrorInvalidValue;
+    if (!qj.blocks) return hipErrorInvalidValue;
   }
   auto by_g = [&](auto t, auto b) -> hipError_t {
     using T = decltype(t);
