@@ -133,7 +133,7 @@ hipError_t launch_prefill(const kvq_rows* q, const kvq_qtensor* k, const kvq_qte
                           float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, causal);
   PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl,
-                               D == 96 || tree);
+                               D == 96);
   quant_operands(p, k, v);
   if (tree) {
     p.tree = tree_params(tree, L);
@@ -148,7 +148,7 @@ hipError_t launch_prefill_paged(const kvq_rows* q, const kvq_qtensor* k, const k
                                 int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, causal);
   PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl,
-                               D == 96 || tree);
+                               D == 96);
   quant_operands(p, k, v);  // (batch strides are page strides)
   p.table = table;
   p.table_stride = table_stride;
@@ -164,7 +164,7 @@ hipError_t launch_prefill_dense(const kvq_rows* q, const kvq_rows* k, const kvq_
                                 const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int dtype,
                                 float scale, int causal, int window, void* workspace, hipStream_t stream, const kvq_tree* tree) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, causal);
-  PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl, D == 64 || tree);
+  PreParams p = prefill_params(q, seq_lens, out, Hq, Hkv, L, D, S, scale, causal, window, workspace, pl, D == 64);
   dense_operands(p, k, v);
   p.out8 = ((uintptr_t)out->data % 16 || (out->stride_b | out->stride_h | out->stride_l) % 8) ? 1 : 0;
   if (tree) {
@@ -177,10 +177,10 @@ hipError_t launch_prefill_dense(const kvq_rows* q, const kvq_rows* k, const kvq_
   return bf ? launch_prefill_t<BF16, 16>(p, stream) : launch_prefill_t<F16, 16>(p, stream);
 }
 
-// ---- trees of drafted tokens (prefill_tree.hip): the plan of a call without a causal mask, fp32 partials
+// ---- trees of drafted tokens (prefill_tree.hip): the plan of a call without a causal mask
 size_t prefill_tree_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window) {
   const PrePlan pl = prefill_plan(B, Hq, Hkv, L, S, window, 0);
-  return pl.nsplit > 1 ? prefill_layout(pl, D, true).total : kCounterBytes;
+  return pl.nsplit > 1 ? prefill_layout(pl, D, D != 128).total : kCounterBytes;
 }
 
 // ---- general masks (prefill_masked.hip)

@@ -487,10 +487,9 @@ __device__ __forceinline__ void stage_v_raw(const uint8_t* raw, _Float16* vlds, 
 
 // Whether a split's partial rows are kept in fp32: for the calls that kernels with fp32 partials served before
 // this one (head_dim 96 and general masks the decode kernel, unquantized head_dim 64 the head_dim-256
-// kernel's form of that width), and for trees of drafted tokens. The others pack them to fp16, which their
-// workspaces are sized for.
-template <int BITS, int D, int MASKED, bool TREE = false>
-constexpr bool kF32Partials = MASKED != 0 || TREE || D == 96 || (BITS == 16 && D == 64);
+// kernel's form of that width). The others pack them to fp16, which their workspaces are sized for.
+template <int BITS, int D, int MASKED>
+constexpr bool kF32Partials = MASKED != 0 || D == 96 || (BITS == 16 && D == 64);
 
 // MASKED: 0, or under a general mask: 1 boolean, 2 additive. The tile loop then walks the list of tiles
 // with a visible key, and reads the mask beside those that are not visible as a whole.
@@ -1170,7 +1169,7 @@ __global__ __launch_bounds__(kPW * 64, 1) void prefill_attn_kernel(PreParams p) 
     //    Record of row r at byte 16 (s * kPRows + r) of the unit's record block.
     //  * With fp32 partials (kF32Partials) a row is o itself in the cache's units, word u (0 .. 2 QW - 1) value
     //    group u, and its record (m, l), 8 bytes: the merge scales row s by w_s.
-    constexpr bool F32P = kF32Partials<BITS, D, MASKED, TREE>;
+    constexpr bool F32P = kF32Partials<BITS, D, MASKED>;
     constexpr int NW = F32P ? 2 * QW : QW;       // 16-byte words of a lane's row
     constexpr uint32_t split_o = kPW * NW * 1024;
     const __amdgpu_buffer_rsrc_t ro =

@@ -10,8 +10,9 @@ static hipError_t launch_tree_t(const PreParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((prefill_attn_kernel<T, BITS, PAGED, G, D, 0, true>), dim3(prefill_grid(p)), dim3(kPW * 64), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.nsplit == 1 || p.fused) return e;
-  hipLaunchKernelGGL((prefill_combine_kernel<T, D, true, false, true>), dim3(p.nunits * kPW * (D / 8)), dim3(kPW * 64), 0,
-                     stream, p);
+  constexpr bool f32 = kF32Partials<BITS, D, 0>;
+  hipLaunchKernelGGL((prefill_combine_kernel<T, D, f32, false, true>), dim3(p.nunits * kPW * (D / (f32 ? 8 : 16))),
+                     dim3(kPW * 64), 0, stream, p);
   return hipGetLastError();
 }
 

@@ -23,22 +23,36 @@ __global__ __launch_bounds__(256) void draft_tree_kernel(const int32_t* parents,
   __syncthreads();
   const int l = blockIdx.x * blockDim.x + threadIdx.x;
   if (l >= L) return;
-  int depth = -1, j = l;
-  while (j >= 0) {
-    ++depth;
-    j = par[j];
-  }
-  const bool here = j == -1;
   const int words = (L + 31) / 32;
   uint32_t* row = bits + ((int64_t)b * L + l) * words;
-  j = here ? l : -1;
-  for (int w = words - 1; w >= 0; --w) {
-    uint32_t x = 0;
-    while (j >= 32 * w) {
-      x |= 1u << (j & 31);
+  int depth = -1, j = l;
+  bool here;
+  if (L <= 64) {  // one walk: the row fits a register
+    uint64_t seen = 0;
+    while (j >= 0) {
+      ++depth;
+      seen |= 1ull << j;
       j = par[j];
     }
-    row[w] = x;
+    here = j == -1;
+    if (!here) seen = 0;
+    row[0] = (uint32_t)seen;
+    if (words == 2) row[1] = (uint32_t)(seen >> 32);
+  } else {
+    while (j >= 0) {
+      ++depth;
+      j = par[j];
+    }
+    here = j == -1;
+    j = here ? l : -1;
+    for (int w = words - 1; w >= 0; --w) {
+      uint32_t x = 0;
+      while (j >= 32 * w) {
+        x |= 1u << (j & 31);
+        j = par[j];
+      }
+      row[w] = x;
+    }
   }
   depths[(int64_t)b * L + l] = here ? depth : -1;
   if (positions) positions[(int64_t)b * L + l] = (int32_t)((starts ? starts[b] : start) + (here ? depth : 0));
