@@ -259,14 +259,13 @@ const int32_t* ints_of(PyObject* o, int64_t n, const at::Device& dev) {
   return (const int32_t*)t.data_ptr();
 }
 
-// A block table [B, pages] on `dev` with contiguous rows.
+// A block table [B, pages] on `dev` whose rows follow each other.
 bool table_of(PyObject* o, int64_t B, const at::Device& dev, const int32_t** data, int64_t* stride, int64_t* pages) {
   if (!THPVariable_Check(o)) return false;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (t.scalar_type() != at::kInt || t.device() != dev || t.dim() != 2 || t.size(0) != B || t.stride(1) != 1) return false;
+  if (t.scalar_type() != at::kInt || t.device() != dev || t.dim() != 2 || t.size(0) != B || !t.is_contiguous()) return false;
   *data = (const int32_t*)t.data_ptr();
-  *stride = t.stride(0);
-  *pages = t.size(1);
+  *stride = *pages = t.size(1);
   return true;
 }
 

@@ -1152,6 +1152,13 @@ def _check_table(block_tables: torch.Tensor, B: int, dev) -> None:
         raise ValueError("block_tables must be on the queries' device with contiguous rows")
 
 
+def _whole_table(block_tables: torch.Tensor, B: int, dev) -> torch.Tensor:
+    """A checked table whose rows follow each other: the library takes the distance of its rows for their length, so
+    a view of a wider table's first pages is copied, lest the entries behind it be taken for the sequence's."""
+    _check_table(block_tables, B, dev)
+    return block_tables if block_tables.stride(0) == block_tables.shape[1] else block_tables.contiguous()
+
+
 def paged_quantize_append(k: torch.Tensor, k_pool: Triple, v: Optional[torch.Tensor], v_pool: Optional[Triple],
                           block_tables: torch.Tensor, *, starts: Optional[torch.Tensor] = None, row_offset: int = 0,
                           group_size: int = 64, bits: int = 8, rope: Optional[Rope] = None) -> None:
@@ -1205,7 +1212,7 @@ def paged_rope_axes_append(k: torch.Tensor, k_pool: Triple, v: Optional[torch.Te
     rp, B, H, L, D = call._check(k, v, positions, queries)
     if k_pool[0].shape[1] != H or k_pool[0].shape[2] != PAGE_ROWS:
         raise ValueError(f"pools must be [num_pages, {H}, {PAGE_ROWS}, *]")
-    _check_table(block_tables, B, call._dev)
+    block_tables = _whole_table(block_tables, B, call._dev)
     call._launch(k, v, queries, rp, B, H, L, D, row_offset,
                  (k_pool[0].shape[0], block_tables.data_ptr(), block_tables.stride(0), _check_starts(starts, B, call._dev)))
 
@@ -1225,7 +1232,7 @@ def paged_dequantize(k_pool: Triple, v_pool: Optional[Triple], block_tables: tor
     if rows != PAGE_ROWS:
         raise ValueError(f"pools must be [num_pages, H, {PAGE_ROWS}, *]")
     B = block_tables.shape[0]
-    _check_table(block_tables, B, dev)
+    block_tables = _whole_table(block_tables, B, dev)
     if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,) or seq_lens.device != dev or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous int32 tensor of B entries on the pools' device")
     if max_len is None:
@@ -1316,7 +1323,7 @@ def paged_keep_rows(pools: Sequence[Tuple[Triple, Triple]], block_tables: torch.
     tensors = [t for layer in pools for tr in layer for t in tr]
     B = block_tables.shape[0]
     dev, H, M, sb = _check_kept(tensors, rows, B, n)
-    _check_table(block_tables, B, dev)
+    block_tables = _whole_table(block_tables, B, dev)
     pages = tensors[0].shape[0]
     if any(t.shape[0] != pages or t.shape[2] != PAGE_ROWS for t in tensors):
         raise ValueError(f"pools must be [{pages}, H, {PAGE_ROWS}, *]")
@@ -1369,6 +1376,7 @@ def paged_attention(queries: torch.Tensor, k_pool: Triple, v_pool: Triple, block
         queries = _copy_for_one_shot(queries, "queries", True)
     out = _check_out(out, queries, dev)
     if tree is not None:
+        block_tables = _whole_table(block_tables, B, dev)
         _check_tree_call(tree, B, L, S, window, causal, kernel, dev)
         nbytes, _ = _tree_sizes(B, Hq, Hkv, L, D, S, int(group_size), int(window))
         if nbytes == 0:

@@ -178,6 +178,38 @@ def test_keeps_paged_rows(monkeypatch):
     assert not same(got, [x.nan_to_num(3) if x.is_floating_point() else x for x in (*kp, *vp)])
 
 
+def test_tables_that_are_views():
+    """The first pages of a wider table, whose other entries name pages of somebody else: rows past the view are
+    dropped, and nothing there is read."""
+    from tests.test_gpu_paged import build
+
+    lens = [130, 70]
+    _, table, kp, vp, kc, vc = build(2, 4, lens, 128, 8, torch.float16, 555, npages=20)
+    P = table.shape[1]
+    mine = set(int(x) for b, n in enumerate(lens) for x in table[b, : -(-n // 64)])
+    others = [p for p in range(20) if p not in mine]
+    wide = torch.full((2, 8), others[0], dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + P] = table
+    view = wide[:, 2:2 + P]
+    before = [bits_of(x)[others] for x in (*kp, *vp)]
+    q = seeded_normal((2, 8, 5, 128), 556, torch.float16, DEV)
+    tree = kernels.DraftTree(ints(make_parents("random", 2, 5, 557)))
+    seq = ints(lens)
+    assert torch.equal(kernels.paged_attention(q, kp, vp, view, seq, 0.1, tree=tree),
+                       kernels.paged_attention(q, kp, vp, table, seq, 0.1, tree=tree))
+    with pytest.raises(ValueError):  # rows that the view does not hold
+        kernels.paged_attention(q, kp, vp, view, seq, 0.1, tree=tree, max_len=64 * P + 1)
+    with pytest.raises(ValueError):
+        kernels.paged_dequantize(kp, vp, view, seq, max_len=64 * P + 1)
+    got = kernels.paged_dequantize(kp, vp, view, seq)
+    assert got[0].shape[2] == 64 * P and torch.equal(got[0][0, :, :130], kernels.dequantize_rows(kc, vc)[0][0, :, :130])
+    # rows kept, and appended, across the end of the view
+    kernels.paged_keep_rows([(kp, vp)], view, ints([1, 3]), starts=ints([64 * P - 1, 64 * P - 2]))
+    k = seeded_normal((2, 4, 4, 128), 558, torch.float16, DEV)
+    kernels.paged_rope_axes_append(k, kp, k, vp, view, kernels.RopeAxes(128), ints([[0, 1, 2, 3]]), starts=ints([64 * P - 2] * 2))
+    assert all(torch.equal(bits_of(x)[others], y) for x, y in zip((*kp, *vp), before))
+
+
 def test_handed_back():
     """Forms that the Python path serves (or refuses) as before: rows to copy, triples as lists, K alone."""
     kt, vt = make_cache(1, 4, 300, 128, 8, torch.float16, 560)
