@@ -753,7 +753,7 @@ static int check_tree(const kvq_tree* t, int L, float scale, int window) {
 // less than 2^25 elements; the prefill kernel (256 rows a pass) once the rows kernel's blocks of 32 past the fourth
 // read more than 2^25. us, decode / rows / prefill (head_dim 128, groups of 64, 8 KV heads unless said):
 //   20 rows,  4106 keys  11.5 / 13.8 /  22    32 rows, 8 sequences of 4096, 4 bits  32.5 / 26.2 / 53.0
-//   24 rows, 16384 keys  20.1 / 25.8 /  32    64 rows, 8 sequences of 6144, 4 bits  68.9 / 41.7 / 71.8
+//   24 rows, 16384 keys  20.1 / 25.8 /  32    64 rows, 8 sequences of 6144, 4 bits  68.9 / 40.3 / 71.8
 //   64 rows,  4096 keys  14.5 / 13.8 /  21   128 rows, 32768 keys                    116 / 48.8 / 53.6
 //   64 rows,  8192 keys  21.6 / 18.7 /  25   192 rows, 32768 keys                    215 / 65.7 / 56.4
 //  256 rows,  2048 keys  20.6 / 20.7 /  24   256 rows, 32768 keys                    215 / 79.9 / 59.6

@@ -13,8 +13,8 @@
 //    The lane halves take halves of the row (dims hh D/2 + 8j in k-step j), which the query operand follows.
 //  * Every lane then holds 16 scores of one row: maximum and sum are lane-local, and the packed probabilities are the
 //    B operand of O^T = V^T P^T.
-//  * V^T: lane n owns dims (D/32) n .. of 8 keys a k-step; byte permutes pair neighbouring keys, and packed FMAs apply
-//    their scales and biases, which the wave's lanes converted once per tile into a small table.
+//  * V^T: lane n owns dims (D/32) n .. of 8 keys a k-step; byte permutes (4 bits: masks) pair neighbouring keys, and
+//    packed FMAs apply their scales and biases, which the wave's lanes converted once per tile into a small table.
 //  * Splits are merged as the decode kernel's are: up to 4 by the last to finish, more by combine_kernel.
 // Operands and roundings are the prefill kernel's: q times a power of two in fp16 (exact), K and V dequantized to fp16
 // (a bf16 cache's times 2^-E), probabilities in fp16, everything else in fp32; an unquantized cache runs in its own
@@ -23,8 +23,9 @@
 //
 // Measured with the merge (decode kernel / here / prefill kernel, us): 8 KV heads over 32768 keys of 128 dims in 8 bits
 // (75 MB, 14.5 us as a copy), 32 rows 38.7 / 31.3 / 51.0, 64 rows 64.5 / 32.7 / 50.8, 128 rows 116 / 48.8 / 53.6;
-// 8 sequences of 6144 keys in 4 bits, 64 rows 68.9 / 41.7 / 71.8. Bound by instruction issue: a tile is about 320 vector
-// and 80 scalar instructions for 24 MFMAs, the vector ALUs are busy 70% of the cycles at 512 rows. Blocks of 64 rows
+// 8 sequences of 6144 keys in 4 bits, 64 rows 68.9 / 40.3 / 71.8. Bound by the vector ALUs, 75% busy at 512 rows: a tile
+// is about 320 vector instructions (16 of them exponentials, four times as long) and 80 scalar ones beside 24 MFMAs;
+// calls of few tiles a wave (the second, 12) spend as long again before and after them. Blocks of 64 rows
 // (dequantized once for two) came to 35.0 us at 64 rows, 47.3 at 128: one wave a SIMD then hides less than the second
 // block saves. tree_kernel_of (capi.hip) has the rule between the three.
 
@@ -105,6 +106,19 @@ __device__ __forceinline__ uint32_t as_u32(h2 x) { return __builtin_bit_cast(uin
 __device__ __forceinline__ uint32_t dequant_bytes(uint32_t bytes, uint32_t sel, uint32_t s2, uint32_t b2) {
   const h2 x = as_h2(perm(0x64646464u, bytes, sel)) - h2{(_Float16)1024.0f, (_Float16)1024.0f};
   return as_u32(x * as_h2(s2) + as_h2(b2));
+}
+
+// 4-bit codes of a word's two halves, nibbles 0 .. 3 of each: out[i] is the pair of nibbles i, dequantized. In the mantissa
+// of 1024 a nibble at bits 4 .. 7 counts 16 times: (1024 + 16 c) / 16 - 64 is c, exact.
+__device__ __forceinline__ void dequant_nibbles(uint32_t w, uint32_t s2, uint32_t b2, uint32_t (&out)[4]) {
+  constexpr uint32_t M = 0x64006400u;
+  const h2 one = {(_Float16)-1024.0f, (_Float16)-1024.0f}, six = {(_Float16)0.0625f, (_Float16)0.0625f},
+           off = {(_Float16)-64.0f, (_Float16)-64.0f};
+  const uint32_t w8 = w >> 8;
+  const h2 c[4] = {as_h2((w & 0x000F000Fu) | M) + one, as_h2((w & 0x00F000F0u) | M) * six + off,
+                   as_h2((w8 & 0x000F000Fu) | M) + one, as_h2((w8 & 0x00F000F0u) | M) * six + off};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = as_u32(c[i] * as_h2(s2) + as_h2(b2));
 }
 
 template <typename T>
@@ -287,6 +301,14 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
       for (int i = 0; i < 4; ++i)
         qop[j][i] = pack_f16x2(to_float((uint16_t)(qop[j][i] & 0xffffu), T{}) * qmul,
                                to_float((uint16_t)(qop[j][i] >> 16), T{}) * qmul);
+    if constexpr (BITS == 4) {  // the dims in the order of dequant_nibbles
+#pragma unroll
+      for (int j = 0; j < C::KSTEPS; ++j) {
+        const u4 q = qop[j];
+        qop[j] = u4{perm(q[2], q[0], 0x05040100u), perm(q[2], q[0], 0x07060302u), perm(q[3], q[1], 0x05040100u),
+                    perm(q[3], q[1], 0x07060302u)};
+      }
+    }
   }
 
   const int lo_all = p.window > 0 ? max(0, S_b - p.window) : 0;
@@ -405,10 +427,9 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
             a = u4{dequant_bytes(w0, 0x04010400u, ks2[g], kb2[g]), dequant_bytes(w0, 0x04030402u, ks2[g], kb2[g]),
                    dequant_bytes(w1, 0x04010400u, ks2[g], kb2[g]), dequant_bytes(w1, 0x04030402u, ks2[g], kb2[g])};
           } else {
-            const uint32_t w = kraw[j / 4][j % 4], lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
-            const uint32_t x0 = perm(hi, lo, 0x05010400u), x1 = perm(hi, lo, 0x07030602u);  // dims 0..3, 4..7
-            a = u4{dequant_bytes(x0, 0x04010400u, ks2[g], kb2[g]), dequant_bytes(x0, 0x04030402u, ks2[g], kb2[g]),
-                   dequant_bytes(x1, 0x04010400u, ks2[g], kb2[g]), dequant_bytes(x1, 0x04030402u, ks2[g], kb2[g])};
+            uint32_t x[4];  // dims (0, 4), (1, 5), (2, 6), (3, 7)
+            dequant_nibbles(kraw[j / 4][j % 4], ks2[g], kb2[g], x);
+            a = u4{x[0], x[1], x[2], x[3]};
           }
         }
         s = mfma_32x32x16(a, qop[j], s, OT{});
@@ -442,19 +463,19 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
             vop[t][1][a] = perm(y.w, x.w, 0x07060302u);
           }
         } else {
-          // two keys' codes of two dims as bytes: (x d0, y d0, x d1, y d1)
           const uint32_t s2 = vs[t][a >> 1][a & 1], b2 = vb[t][a >> 1][a & 1], x = vraw[t][2 * a].w, y = vraw[t][2 * a + 1].w;
+          if constexpr (BITS == 8) {  // two keys' codes of two dims as bytes: (x d0, y d0, x d1, y d1)
 #pragma unroll
-          for (int d = 0; d < C::DPL; d += 2) {
-            uint32_t xy;
-            if constexpr (BITS == 8) {
-              xy = perm(y, x, d == 0 ? 0x05010400u : 0x07030602u);
-            } else {
-              const uint32_t both = x | (y << 16);  // 16 bits of each: nibble d is dim d
-              xy = perm((both >> (4 * d + 4)) & 0x000F000Fu, (both >> (4 * d)) & 0x000F000Fu, 0x06040200u);
+            for (int d = 0; d < C::DPL; d += 2) {
+              const uint32_t xy = perm(y, x, d == 0 ? 0x05010400u : 0x07030602u);
+              vop[t][d][a] = dequant_bytes(xy, 0x04010400u, s2, b2);
+              vop[t][d + 1][a] = dequant_bytes(xy, 0x04030402u, s2, b2);
             }
-            vop[t][d][a] = dequant_bytes(xy, 0x04010400u, s2, b2);
-            vop[t][d + 1][a] = dequant_bytes(xy, 0x04030402u, s2, b2);
+          } else {  // DPL nibbles of each
+            uint32_t v4[4];
+            dequant_nibbles(x | (y << 16), s2, b2, v4);
+#pragma unroll
+            for (int d = 0; d < C::DPL; ++d) vop[t][d][a] = v4[d];
           }
         }
       }
