@@ -357,6 +357,7 @@ class QuantizedKVCache:
         words = [kernels.range_exponent(tuple(x[:, :, :rows] for x in tr), self.bits) for tr in (keys, values)]
         self.keys, self.values, self.offset = tuple(keys), tuple(values), int(rows)
         self.range_exp = torch.cat(words)
+        self._append_key = self._axes_key = None  # (prepared appends raise the word that was registered before)
         kernels.register_range_word(self.keys[0], self.range_exp[0:1])
         kernels.register_range_word(self.values[0], self.range_exp[1:2])
 

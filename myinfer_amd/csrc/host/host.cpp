@@ -471,9 +471,10 @@ PyObject* rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
-// axes_append(state address, keys, values, positions, row_offset, queries or None, stream) -> as append()
+// axes_append(state address, keys, values, positions, row_offset, queries or None, stream, block table or None, starts or
+// None) -> as append(); with a block table the state's destination is a pool (B: its pages, rows: a page's)
 PyObject* axes_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7 || !d.axes_append || !THPVariable_Check(a[1]) || !THPVariable_Check(a[2])) return none();
+  if (n != 9 || !d.axes_append || !THPVariable_Check(a[1]) || !THPVariable_Check(a[2])) return none();
   try {
     const AppendState* st = (const AppendState*)PyLong_AsVoidPtr(a[0]);
     const long long row = PyLong_AsLongLong(a[4]);
@@ -487,24 +488,33 @@ PyObject* axes_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (dtype_code(k.scalar_type()) != st->code || v.scalar_type() != k.scalar_type() || !st->vq) return none();
     kvq_rows kr, vr, qr;
     if (k.numel() == 0 || !rows_of(k, &kr) || !rows_of(v, &vr) || k.sizes() != v.sizes()) return none();
-    const int64_t L = k.size(2), D = k.size(3);
-    if (k.size(0) != st->B || k.size(1) != st->H || row < 0 || row + L > st->rows || L > INT32_MAX) return none();
+    const int64_t B = k.size(0), L = k.size(2), D = k.size(3);
+    const bool paged = a[7] != Py_None;
+    int64_t table_stride = 0, pages = 0;
+    const int32_t *table = nullptr, *starts = nullptr;
+    if (k.size(1) != st->H || row < 0 || !fits_int({B, L}) || (!paged && (B != st->B || row + L > st->rows))) return none();
+    if (paged) {
+      if (st->rows != KVQ_PAGE_ROWS || !table_of(a[7], B, k.device(), &table, &table_stride, &pages)) return none();
+      if (a[8] != Py_None && !(starts = ints_of(a[8], B, k.device()))) return none();
+    } else if (a[8] != Py_None) {
+      return none();
+    }
     if (D * st->bits / 32 != st->code_words || D / st->group != st->groups) return none();
     int64_t Hq = 0;
     if (a[5] != Py_None) {
       if (!THPVariable_Check(a[5])) return none();
       const at::Tensor& q = THPVariable_Unpack(a[5]);
       if (q.numel() == 0 || q.scalar_type() != k.scalar_type() || q.device() != k.device() || !rows_of(q, &qr)) return none();
-      if (q.size(0) != st->B || q.size(2) != L || q.size(3) != D || !fits_int({q.size(1)})) return none();
+      if (q.size(0) != B || q.size(2) != L || q.size(3) != D || !fits_int({q.size(1)})) return none();
       Hq = q.size(1);
     }
     kvq_axes ax = *(const kvq_axes*)st->rope;
-    if (!positions_of(a[3], st->B, L, k.device(), &ax)) return none();
+    if (!positions_of(a[3], B, L, k.device(), &ax)) return none();
     int rc;
     {
       Unlocked u;
-      rc = d.axes_append(&kr, st->kq, &vr, st->vq, Hq ? &qr : nullptr, (int)Hq, &ax, 0, nullptr, 0, nullptr, row, (int)st->B,
-                         (int)st->H, (int)L, (int)D, st->bits, st->group, st->code, stream);
+      rc = d.axes_append(&kr, st->kq, &vr, st->vq, Hq ? &qr : nullptr, (int)Hq, &ax, table ? (int)st->B : 0, table,
+                         table_stride, starts, row, (int)B, (int)st->H, (int)L, (int)D, st->bits, st->group, st->code, stream);
     }
     if (rc != KVQ_OK) return failed(rc);
     Py_RETURN_TRUE;

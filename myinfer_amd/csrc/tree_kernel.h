@@ -390,6 +390,8 @@ __global__ __launch_bounds__(kTW * 64, (TreeCfg<D, BITS, G>::MINWG)) void tree_a
       for (int e = 0; e < 8; ++e) vraw[t][e].load(sl + off_v + (16 * t + 8 * (e >> 2) + (e & 3)) * C::ROWB);
     u2 vs[2][2], vb[2][2];  // scales and biases of the 8 keys of k-step t: keys 16 t + 4 hh .. + 3, and + 8
     if constexpr (!C::DENSE) {
+      // (a wave's LDS operations keep their order; the compiler's must too, across the types)
+      asm volatile("" ::: "memory");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int t = 0; t < 2; ++t)

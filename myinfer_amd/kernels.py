@@ -233,8 +233,9 @@ def rope_axes(x: torch.Tensor, r: RopeAxes, positions: torch.Tensor) -> torch.Te
 
 
 class AxesAppendCall:
-    """A quantize-append into fixed destination buffers, with the rotation of the step's keys and queries at given
-    positions, its descriptors built once (``prepare_axes_append``). Launches on the stream current at the call."""
+    """A quantize-append into fixed destination buffers, or with ``paged`` into the pages of fixed pools, with the rotation
+    of the step's keys and queries at given positions, its descriptors built once (``prepare_axes_append``). Launches on the
+    stream current at the call."""
 
     def __init__(self, k_dst: Triple, v_dst: Optional[Triple], rope: RopeAxes, group_size: int, bits: int):
         _check_triple(k_dst, "k_dst")
@@ -245,7 +246,8 @@ class AxesAppendCall:
             if any(tuple(a.shape) != tuple(b.shape) for a, b in zip(k_dst, v_dst)) or v_dst[1].dtype != k_dst[1].dtype:
                 raise ValueError("k_dst and v_dst must have the same shapes and dtype")
         self._dev = _require_cuda(*tens)
-        self._keep = (k_dst, v_dst)
+        # (the range words are held too: the descriptors point to them)
+        self._keep = (k_dst, v_dst, range_word(k_dst[0]), None if v_dst is None else range_word(v_dst[0]))
         codes, scales, _ = k_dst
         if tuple(scales.shape[:3]) != tuple(codes.shape[:3]):
             raise ValueError("the destination's codes and scales must have the same rows")
@@ -255,6 +257,7 @@ class AxesAppendCall:
         self._vq = None if v_dst is None else _lib.qtensor(*v_dst, range_exp=range_word(v_dst[0]))
         self._dtype, self._code = scales.dtype, _lib.dtype_code(scales.dtype)
         self._bits, self._group = int(bits), int(group_size)
+        self.rope = rope
         self._rp = rope.params()
         self._state = _lib.AppendState(
             None, ctypes.addressof(self._kq), None if self._vq is None else ctypes.addressof(self._vq),
@@ -296,19 +299,35 @@ class AxesAppendCall:
 
     def __call__(self, k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, row_offset: int,
                  queries: Optional[torch.Tensor] = None) -> None:
-        host, stream = _native(k)
-        if host is not None:
-            done = host.axes_append(self._state_ptr, k, v, positions, row_offset, queries, stream)
-            if done is True:
-                return
-            if done is not None:
-                _lib.check(done, "kvq_rope_axes_append")
+        if self._native_append(k, v, positions, row_offset, queries, None, None):
+            return
         rp, B, H, L, D = self._check(k, v, positions, queries)
         if (B, H) != self._lead:
             raise ValueError(f"destination leads {self._lead} do not match source {(B, H)}")
         if row_offset < 0 or row_offset + L > self._rows:
             raise ValueError(f"rows [{row_offset}, {row_offset + L}) exceed the destination's {self._rows} rows")
         self._launch(k, v, queries, rp, B, H, L, D, row_offset, (0, None, 0, None))
+
+    def paged(self, k: torch.Tensor, v: Optional[torch.Tensor], positions: torch.Tensor, block_tables: torch.Tensor,
+              starts: Optional[torch.Tensor] = None, row_offset: int = 0, queries: Optional[torch.Tensor] = None) -> None:
+        """``paged_rope_axes_append`` into the prepared pools."""
+        if self._native_append(k, v, positions, row_offset, queries, block_tables, starts):
+            return
+        rp, B, H, L, D = self._check(k, v, positions, queries)
+        if self._lead[1] != H or self._rows != PAGE_ROWS:
+            raise ValueError(f"pools must be [num_pages, {H}, {PAGE_ROWS}, *]")
+        block_tables = _whole_table(block_tables, B, self._dev)
+        self._launch(k, v, queries, rp, B, H, L, D, row_offset,
+                     (self._lead[0], block_tables.data_ptr(), block_tables.stride(0), _check_starts(starts, B, self._dev)))
+
+    def _native_append(self, k, v, positions, row_offset, queries, table, starts) -> bool:
+        host, stream = _native(k)
+        if host is None:
+            return False
+        done = host.axes_append(self._state_ptr, k, v, positions, row_offset, queries, stream, table, starts)
+        if done is not None and done is not True:
+            _lib.check(done, "kvq_rope_axes_append")
+        return done is True
 
 
 def prepare_axes_append(k_dst: Triple, v_dst: Optional[Triple] = None, *, rope: RopeAxes, group_size: int = 64,
@@ -1208,13 +1227,7 @@ def paged_rope_axes_append(k: torch.Tensor, k_pool: Triple, v: Optional[torch.Te
                            queries: Optional[torch.Tensor] = None, group_size: int = 64, bits: int = 8) -> None:
     """``paged_quantize_append`` with the keys rotated at `positions` (int32 [axes, B, L]) first, and the rows of
     `queries` [B, Hq, L, D] rotated in place in the same launch."""
-    call = AxesAppendCall(k_pool, v_pool, rope, group_size, bits)
-    rp, B, H, L, D = call._check(k, v, positions, queries)
-    if k_pool[0].shape[1] != H or k_pool[0].shape[2] != PAGE_ROWS:
-        raise ValueError(f"pools must be [num_pages, {H}, {PAGE_ROWS}, *]")
-    block_tables = _whole_table(block_tables, B, call._dev)
-    call._launch(k, v, queries, rp, B, H, L, D, row_offset,
-                 (k_pool[0].shape[0], block_tables.data_ptr(), block_tables.stride(0), _check_starts(starts, B, call._dev)))
+    AxesAppendCall(k_pool, v_pool, rope, group_size, bits).paged(k, v, positions, block_tables, starts, row_offset, queries)
 
 
 def paged_dequantize(k_pool: Triple, v_pool: Optional[Triple], block_tables: torch.Tensor, seq_lens: torch.Tensor, *,

@@ -119,6 +119,7 @@ class PagedRadixKVCache:
 
         self._k = [pool() for _ in range(num_layers)]
         self._v = [pool() for _ in range(num_layers)]
+        self._axes: dict = {}  # layer -> its prepared append at positions
 
     # ---- the reference's interface (native/include/kv_cache.hpp:28-54)
 
@@ -182,9 +183,11 @@ class PagedRadixKVCache:
         if isinstance(rope, kernels.RopeAxes):
             if positions is None:
                 raise ValueError("a kernels.RopeAxes needs positions")
-            kernels.paged_rope_axes_append(keys, self._k[layer], values, self._v[layer], block_tables, rope, positions,
-                                           starts=starts, row_offset=row_offset, queries=queries,
-                                           group_size=self.group_size, bits=self.bits)
+            call = self._axes.get(layer)
+            if call is None or call.rope != rope:  # the layer's descriptors, built once
+                call = self._axes[layer] = kernels.prepare_axes_append(self._k[layer], self._v[layer], rope=rope,
+                                                                       group_size=self.group_size, bits=self.bits)
+            call.paged(keys, values, positions, block_tables, starts, row_offset, queries)
             return
         if positions is not None or queries is not None:
             raise ValueError("positions and queries go with a kernels.RopeAxes")

@@ -178,6 +178,28 @@ def test_keeps_paged_rows(monkeypatch):
     assert not same(got, [x.nan_to_num(3) if x.is_floating_point() else x for x in (*kp, *vp)])
 
 
+@pytest.mark.parametrize("starts,queries", [(True, True), (False, False)])
+def test_paged_append(monkeypatch, starts, queries):
+    from myinfer_amd.paged import PagedRadixKVCache
+
+    r = kernels.RopeAxes(128, (16, 24, 24))
+    k, v = (seeded_normal((2, 4, 9, 128), 580 + i, torch.bfloat16, DEV) for i in range(2))
+    pos = torch.randint(0, 500, (3, 2, 9), dtype=torch.int32, device=DEV)
+
+    def run():
+        pool = PagedRadixKVCache(1, 4, 128, 8, dtype=torch.bfloat16, device=DEV)
+        q = seeded_normal((2, 8, 9, 128), 582, torch.bfloat16, DEV)
+        table = ints([[5, 2], [0, 7]])
+        for step in range(2):  # (the second with the first's descriptors)
+            pool.append(0, k, v, table, starts=ints([60, 3 + step]) if starts else None, row_offset=0 if starts else 50, rope=r,
+                        positions=pos, queries=q if queries else None)
+        return [*pool.k_cache(0), *pool.v_cache(0), q]
+
+    got = run()
+    assert same(got, python_path(monkeypatch, run))
+    assert got[1].any()
+
+
 def test_tables_that_are_views():
     """The first pages of a wider table, whose other entries name pages of somebody else: rows past the view are
     dropped, and nothing there is read."""

@@ -262,3 +262,40 @@ def test_refusals():
         pool.keep_rows(t, ok, torch.zeros(3, dtype=torch.int32, device=DEV))
     with pytest.raises(ValueError, match="kept"):
         pool.keep_rows(t, ok, torch.zeros(2, dtype=torch.int32, device=DEV), n=2)
+
+
+def test_restored_twice_raises_the_registered_word():
+    """Appends after a second restore of the same buffers raise the range word that is registered then, by either
+    append, and the earlier one is left alone."""
+    from myinfer_amd.cache import QuantizedKVCache
+
+    r = kernels.RopeAxes(128)
+    k, v = (seeded_normal((1, 2, 8, 128), 700 + i, torch.bfloat16, DEV) for i in range(2))
+    pos = torch.zeros(1, 8, dtype=torch.int32, device=DEV)
+    for rope in (None, r):
+        kw = {} if rope is None else dict(rope=rope, positions=pos)
+        c = QuantizedKVCache(64, 8)
+        c.reserve(k, 256)
+        keys, values = c.keys, c.values
+        c.restore(keys, values, 0)
+        c.update_and_fetch(k, v, **kw)
+        first = c.range_exp
+        c.restore(keys, values, 8)
+        c.update_and_fetch(k, v * 1e6, **kw)
+        assert c.range_exponents()[1] > 0 and first.tolist() == [0, 0]
+
+
+def test_rows_that_do_not_exist():
+    """Reading and keeping of nothing: no rows, no arrays' change."""
+    from myinfer_amd.cache import QuantizedKVCache, keep_rows as keep_cached
+
+    c = QuantizedKVCache(64, 8)
+    k = seeded_normal((1, 2, 8, 128), 710, torch.float16, DEV)
+    c.update_and_fetch(k, k)
+    before = [bits_of(x).clone() for x in (*c.keys, *c.values)]
+    assert c.dequantized(3, 3)[0].shape == (1, 2, 0, 128)
+    assert keep_cached([c], 8, torch.zeros(1, 0, dtype=torch.int32, device=DEV)) == 8
+    assert keep_cached([c], 5, torch.zeros(0, dtype=torch.int32, device=DEV)) == 5
+    assert all(torch.equal(bits_of(x), y) for x, y in zip((*c.keys, *c.values), before))
+    plain = QuantizedKVCache(64, 8).to_unquantized()
+    assert plain.keys is None and plain.offset == 0
