@@ -156,7 +156,12 @@ inline hipError_t launch_combine(const MergeParams& m, int B, hipStream_t stream
     case 4: hipLaunchKernelGGL((combine_kernel<T, D, 4>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 8: hipLaunchKernelGGL((combine_kernel<T, D, 8>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 16: hipLaunchKernelGGL((combine_kernel<T, D, 16>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
-    case 32: hipLaunchKernelGGL((combine_kernel<T, D, 32>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
+    case 32:
+      if constexpr (D <= 128) {
+        hipLaunchKernelGGL((combine_kernel<T, D, 32>), grid, dim3(256), 0, stream, mm, nrows, dv);
+        break;
+      }
+      return hipErrorInvalidValue;
     case 128: hipLaunchKernelGGL((combine_kernel<T, D, 128>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     default: return hipErrorInvalidValue;
   }

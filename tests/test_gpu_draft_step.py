@@ -117,3 +117,77 @@ def test_steps_over_pages():
             for s in range(B):
                 for x, y in zip(*(p.gather(layer, tables[s].tolist(), int(lens[s])) for p in (drafted, single))):
                     assert all(torch.equal(bits_of(i), bits_of(j)) for i, j in zip(x, y))
+
+
+@pytest.mark.parametrize("L,S", [(6, 300), (24, 1900)])
+def test_captured_steps_over_pages(L, S):
+    """A drafted step captured into a graph (the tree, the append with its queries, attention, the kept rows, reading back),
+    two of them over their own pools, replayed with new inputs in place, by turns and at once: the eager step's results
+    and pools, bit for bit."""
+    print(f"captured draft steps L={L} S={S}", flush=True)
+    B, Hq, Hkv, D, dtype = 4, 64, 8, 128, torch.bfloat16
+    r = kernels.RopeAxes(D, base=1e6)
+    width = -(-(S + L) // 64)
+    tables = torch.randperm(B * width, generator=torch.Generator().manual_seed(5)).view(B, width).to(torch.int32).to(DEV)
+    pools = [PagedRadixKVCache(1, Hkv, D, max_blocks=B * width, dtype=dtype) for _ in range(4)]  # graphs', eager ones
+    k, v = (seeded_normal((B, Hkv, S, D), j, dtype, DEV) for j in range(2))
+    pos = torch.arange(S, dtype=torch.int32, device=DEV)[None]
+    for p in pools:
+        p.append(0, k, v, tables, rope=r, positions=pos)
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        parents = torch.tensor(make_parents("gaps", B, L, seed), dtype=torch.int32)
+        rows = torch.stack([torch.randperm(L, generator=g)[:4].sort()[0] for _ in range(B)]).to(torch.int32)
+        starts = torch.randint(1, S + 1, (B,), generator=g, dtype=torch.int32)
+        new = [seeded_normal(shape, seed + j, dtype, DEV) for j, shape in
+               enumerate([(B, Hkv, L, D), (B, Hkv, L, D), (B, Hq, L, D)])]
+        return [parents.to(DEV), rows.to(DEV), starts.to(DEV), *new]
+
+    def step(pool, tree, rows, starts, k, v, q):
+        tree.refresh()
+        pool.append(0, k, v, tables, starts=starts, rope=r, positions=tree.positions, queries=q)
+        out = pool.attention(0, q, tables, starts + L, 1 / math.sqrt(D), max_len=S + L, tree=tree)
+        pool.keep_rows(tables, rows, starts, L)
+        return [out, q, *pool.dequantized(0, tables, starts + 4, max_len=S + L)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, held = [], []
+    for i in range(2):
+        x = inputs(600 + i)
+        with torch.cuda.stream(side):
+            tree = kernels.DraftTree(x[0], starts=x[2])
+            step(pools[i], tree, x[1], x[2], *x[3:])  # loads the code
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                out = step(pools[i], tree, x[1], x[2], *x[3:])
+        graphs.append(g)
+        held.append((x, out, tree))
+    torch.cuda.synchronize()
+    for i in range(2):  # the eager pools as the graphs' are
+        for a, b in zip((*pools[i].k_cache(0), *pools[i].v_cache(0)), (*pools[2 + i].k_cache(0), *pools[2 + i].v_cache(0))):
+            bits_of(b).copy_(bits_of(a))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        fresh = [inputs(700 + 10 * rep + i) for i in range(2)]
+        for i in range(2):
+            for a, b in zip(held[i][0], fresh[i]):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i] if rep % 2 else torch.cuda.current_stream()):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            x = fresh[i]
+            want = step(pools[2 + i], kernels.DraftTree(x[0], starts=x[2]), x[1], x[2], *x[3:])
+            torch.cuda.synchronize()
+            assert torch.equal(held[i][1][0], want[0]) and torch.equal(held[i][0][5], want[1]), f"replay {rep}, graph {i}"
+            for a, b in zip(held[i][1][2:], want[2:]):
+                for s in range(B):
+                    n = int(x[2][s]) + 4
+                    assert torch.equal(a[s, :, :n], b[s, :, :n])
+            for a, b in zip((*pools[i].k_cache(0), *pools[i].v_cache(0)), (*pools[2 + i].k_cache(0), *pools[2 + i].v_cache(0))):
+                assert torch.equal(bits_of(a), bits_of(b)), f"replay {rep}, pool {i}"
