@@ -314,7 +314,7 @@ int kvq_draft_tree(const int32_t* parents, int64_t parents_stride_b, int B, int 
  *   window:   0 = none; else at least L: keys at positions > the node's position - window only.
  *   scale:    positive.
  * Calls of some tens of rows a KV head and of more run on kernels of their own; those of the most rows read a bf16
- * cache's range words (kvq_tree_reads_range says where), and without them run slower. Hidden keys' values enter a
+ * cache's range words (KVQ_TREE_PREFILL below), and without them run slower. Hidden keys' values enter a
  * product with zero: they have to be finite, as under the other masks. workspace: kvq_tree_workspace_size bytes, 256-byte aligned, zero-filled
  * when it is allocated.
  */
@@ -325,8 +325,14 @@ int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v,
 
 size_t kvq_tree_workspace_size(int B, int Hq, int Hkv, int L, int D, int S, int window);
 
-/* 1 if kvq_tree_attn may take a kernel that reads a bf16 cache's range words at these sizes, else 0. */
-int kvq_tree_reads_range(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window);
+/*
+ * The kernel that a tree call of these sizes takes if its tensors allow it (bits 16: an unquantized cache): the decode
+ * kernel, the one for some tens of query rows a KV head, or the prefill kernels (which read a bf16 cache's range words).
+ */
+#define KVQ_TREE_DECODE 0
+#define KVQ_TREE_ROWS 1
+#define KVQ_TREE_PREFILL 2
+int kvq_tree_kernel(int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int window);
 
 /* The same over an unquantized cache (kvq_decode_attn_dense's arguments and head dims). */
 int kvq_tree_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v, const int32_t* seq_lens,

@@ -132,6 +132,7 @@ _DENSE_MASKED_ARGS = [
 
 
 TREE_MAX_NODES = 1024  # KVQ_TREE_MAX_NODES
+TREE_DECODE, TREE_ROWS, TREE_PREFILL = 0, 1, 2  # KVQ_TREE_*
 
 
 class Tree(ctypes.Structure):
@@ -206,7 +207,7 @@ SIGNATURES = {
     "kvq_tree_attn_dense": (c_int, _DENSE_ARGS[:12] + _TREE_TAIL),
     "kvq_paged_tree_attn": (c_int, _PAGED_ATTN_ARGS[:17] + _TREE_TAIL),
     "kvq_tree_workspace_size": (c_size_t, _WS_ARGS),
-    "kvq_tree_reads_range": (c_int, [c_int] * 8),
+    "kvq_tree_kernel": (c_int, [c_int] * 9),
     "kvq_radix_create": (c_void_p, [c_int, c_int]),
     "kvq_radix_destroy": (None, [c_void_p]),
     "kvq_radix_match_and_allocate": (
@@ -334,7 +335,7 @@ def bind_host(module, *addresses: int) -> None:
 
 # The entry points of a drafted step, in the order the native host path takes them.
 DRAFT_SYMBOLS = ("kvq_draft_tree", "kvq_tree_attn", "kvq_tree_attn_dense", "kvq_paged_tree_attn", "kvq_tree_workspace_size",
-                 "kvq_tree_reads_range", "kvq_rope_axes", "kvq_rope_axes_append", "kvq_dequantize", "kvq_paged_dequantize",
+                 "kvq_tree_kernel", "kvq_rope_axes", "kvq_rope_axes_append", "kvq_dequantize", "kvq_paged_dequantize",
                  "kvq_keep_rows")
 
 _host = None

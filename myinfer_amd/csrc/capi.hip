@@ -748,19 +748,24 @@ static int check_tree(const kvq_tree* t, int L, float scale, int window) {
   return KVQ_OK;
 }
 
-// The kernel of a tree call by its sizes. rows: a KV head's query rows; work: the K elements a pass over the cache reads.
-// head_dim 64 and 128: the decode kernel (16 G / D rows a pass) up to 8 rows and where its passes past the third read
-// less than 2^25 elements; the prefill kernel (256 rows a pass) once the rows kernel's blocks of 32 past the fourth
-// read more than 2^25. us, decode / rows / prefill (head_dim 128, groups of 64, 8 KV heads unless said):
-//   20 rows,  4106 keys  11.5 / 13.8 /  22    32 rows, 8 sequences of 4096, 4 bits  32.5 / 26.2 / 53.0
-//   24 rows, 16384 keys  20.1 / 25.8 /  32    64 rows, 8 sequences of 6144, 4 bits  68.9 / 40.3 / 71.8
-//   64 rows,  4096 keys  14.5 / 13.8 /  21   128 rows, 32768 keys                    116 / 48.8 / 53.6
-//   64 rows,  8192 keys  21.6 / 18.7 /  25   192 rows, 32768 keys                    215 / 65.7 / 56.4
-//  256 rows,  2048 keys  20.6 / 20.7 /  24   256 rows, 32768 keys                    215 / 79.9 / 59.6
-//  124 rows of 64 unquantized dims, 4 sequences of 2047: 11.0 / 11.9 / 22
+// The kernel of a tree call by its sizes: the one whose time is estimated the lowest. rows: a KV head's query rows.
+//   decode: a launch and 25 us (64 dims 18, unquantized 12.5) for a million keys of a pass of 16 G / D rows, and 2.5 for
+//           512 workgroups of it (unquantized 64 dims none);
+//   rows:   its plan's model (tree_attn.hip);
+//   prefill: a launch or two and 85 us (130) for a million keys of a block of 256 rows.
+// Over 260 random calls the choice came to 1.6% more than the best of the three on average (a choice by rows and keys
+// alone 5%), 41% at most. us, decode / rows / prefill (128 dims, groups of 64, 8 bits, 8 KV heads unless said):
+//   20 rows,  4106 keys   11.5 /  13.8 /  22    32 rows, 8 sequences of 4096, 4 bits  32.5 / 26.2 / 53.0
+//   24 rows, 16384 keys   20.1 /  25.8 /  32    64 rows, 8 sequences of 6144, 4 bits  68.9 / 40.3 / 71.8
+//   64 rows,  4096 keys   14.5 /  13.8 /  21   128 rows, 32768 keys                    116 / 48.8 / 53.6
+//   64 rows,  8192 keys   21.6 /  18.7 /  25   192 rows, 32768 keys                    215 / 65.7 / 56.4
+//  256 rows,  2048 keys   20.6 /  20.7 /  24   256 rows, 32768 keys                    215 / 79.9 / 59.6
+//  124 rows of 64 unquantized dims, 4 sequences of 2047: 11.0 / 11.9 / 22; 44 rows of 64 dims, 64 units of 19345: 105 / 60 / 111
+//  928 unquantized rows, 32 units of 265: 90 / 39.5 / 19.3
 // head_dim 96 has no rows kernel, head_dim 256 neither: its prefill kernel's lines are kernels._auto_kernel's.
 enum class TreeKernel { kDecode, kRows, kPrefill };
-static TreeKernel tree_kernel_of(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window, bool dense) {
+static TreeKernel tree_kernel_of(int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int window) {
+  const bool dense = bits == 16;
   const int64_t rows = (int64_t)(Hq / Hkv) * L, units = (int64_t)B * Hkv;
   const int64_t keys = window > 0 ? std::min((int64_t)S, (int64_t)window + L) : S;
   if (D == 96 && !dense) return rows > 64 ? TreeKernel::kPrefill : TreeKernel::kDecode;
@@ -771,21 +776,25 @@ static TreeKernel tree_kernel_of(int B, int Hq, int Hkv, int L, int D, int S, in
     const bool few = rows < 128 && units * passes <= 512 && (passes - 3) * units * keys <= 5 << 15;
     return few ? TreeKernel::kDecode : TreeKernel::kPrefill;
   }
-  const int64_t work = units * keys * D, line = 1 << 25;
-  if ((passes - 3) * work < line) return TreeKernel::kDecode;
-  return ((rows + 31) / 32 - 4) * work > line ? TreeKernel::kPrefill : TreeKernel::kRows;
+  const float work = (float)(units * keys) * 1e-6f;
+  const float pass = D != 64 ? 25.0f : dense ? 12.5f : 18.0f, group = D == 64 && dense ? 0.0f : 2.5f / 512;
+  const float decode = 7.5f + pass * work * passes + group * (float)(units * passes);
+  const float prefill = 14.5f + (D == 64 ? 85.0f : 130.0f) * work * ((rows + 255) / 256);
+  const float mine = kvq::tree_rows_time(B, Hq, Hkv, L, D, S, window, bits);
+  return decode <= mine && decode <= prefill ? TreeKernel::kDecode : mine <= prefill ? TreeKernel::kRows : TreeKernel::kPrefill;
 }
 
-int kvq_tree_reads_range(int B, int Hq, int Hkv, int L, int D, int S, int group_size, int window) {
+int kvq_tree_kernel(int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int window) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || S <= 0 || D <= 0 || window < 0 || group_size <= 0 || Hq % Hkv) return 0;
-  return tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, false) == TreeKernel::kPrefill ? 1 : 0;
+  if (bits == 16) group_size = 64;
+  return (int)tree_kernel_of(B, Hq, Hkv, L, D, S, bits, group_size, window);
 }
 
 // ... and after: what the prefill kernel cannot take (a bf16 cache without range words, output or scale rows that are not
 // aligned for it) runs on the rows kernel, of a width that has none on the decode kernel.
 static TreeKernel tree_kernel_for(const kvq_qtensor* k, const kvq_qtensor* v, const kvq_rows* out, int B, int Hq, int Hkv,
-                                  int L, int D, int S, int group_size, int dtype, int window) {
-  const TreeKernel t = tree_kernel_of(B, Hq, Hkv, L, D, S, group_size, window, k == nullptr);
+                                  int L, int D, int S, int bits, int group_size, int dtype, int window) {
+  const TreeKernel t = tree_kernel_of(B, Hq, Hkv, L, D, S, bits, group_size, window);
   if (t != TreeKernel::kPrefill) return t;
   bool ok = !k || dtype != KVQ_DTYPE_BF16 || (k->range_exp && v->range_exp);
   if (D != 256) {
@@ -810,7 +819,7 @@ int kvq_tree_attn(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v,
   int rc = check_attn(q, k, v, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, window,
                       kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window), workspace, workspace_bytes);
   if (rc || (rc = check_tree(tree, L, scale, window))) return rc;
-  const TreeKernel kernel = tree_kernel_for(k, v, out, B, Hq, Hkv, L, D, S, group_size, dtype, window);
+  const TreeKernel kernel = tree_kernel_for(k, v, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, window);
   hipError_t e;
   if (kernel != TreeKernel::kPrefill) {
     e = kvq::launch_decode(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, scale, 0, window, workspace,
@@ -835,7 +844,7 @@ int kvq_paged_tree_attn(const kvq_rows* q, const kvq_qtensor* k_pool, const kvq_
                             workspace, workspace_bytes);
   if (rc || (rc = check_tree(tree, L, scale, window))) return rc;
   if (!seq_lens) return fail(KVQ_ERR_INVALID, "seq_lens is NULL");
-  const TreeKernel kernel = tree_kernel_for(k_pool, v_pool, out, B, Hq, Hkv, L, D, S, group_size, dtype, window);
+  const TreeKernel kernel = tree_kernel_for(k_pool, v_pool, out, B, Hq, Hkv, L, D, S, bits, group_size, dtype, window);
   hipError_t e;
   if (kernel != TreeKernel::kPrefill) {
     e = kvq::launch_decode_paged(q, k_pool, v_pool, num_pages, block_table, table_stride, seq_lens, out, B, Hq, Hkv, L, D, S,
@@ -858,7 +867,7 @@ int kvq_tree_attn_dense(const kvq_rows* q, const kvq_rows* k, const kvq_rows* v,
   int rc = check_attn_dense(q, k, v, out, B, Hq, Hkv, L, D, S, dtype, scale, window,
                             kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window), workspace, workspace_bytes);
   if (rc || (rc = check_tree(tree, L, scale, window))) return rc;
-  const TreeKernel kernel = tree_kernel_for(nullptr, nullptr, out, B, Hq, Hkv, L, D, S, 64, dtype, window);
+  const TreeKernel kernel = tree_kernel_for(nullptr, nullptr, out, B, Hq, Hkv, L, D, S, 16, 64, dtype, window);
   hipError_t e;
   if (D > 128) {  // unquantized rows past 128 dims run through the head_dim-256 kernel
     e = kvq::launch_wide_dense(q, k, v, seq_lens, out, B, Hq, Hkv, L, D, S, dtype, scale, 0, window, workspace,

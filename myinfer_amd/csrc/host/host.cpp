@@ -47,7 +47,7 @@ struct {
   decltype(&kvq_tree_attn_dense) tree_dense = nullptr;
   decltype(&kvq_paged_tree_attn) tree_paged = nullptr;
   decltype(&kvq_tree_workspace_size) tree_ws = nullptr;
-  decltype(&kvq_tree_reads_range) tree_range = nullptr;
+  decltype(&kvq_tree_kernel) tree_kernel = nullptr;
   decltype(&kvq_rope_axes) rope_axes = nullptr;
   decltype(&kvq_rope_axes_append) axes_append = nullptr;
   decltype(&kvq_dequantize) dequantize = nullptr;
@@ -409,7 +409,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (paged && !lens) return none();
     const int b = (int)B, hq = (int)Hq, hk = (int)Hkv, l = (int)L, dd = (int)D, s = (int)S, w = (int)window;
     if (!dense && !paged && code == KVQ_DTYPE_BF16 && (!kq.range_exp || !vq.range_exp) &&
-        d.tree_range(b, hq, hk, l, dd, s, (int)group, w))
+        d.tree_kernel(b, hq, hk, l, dd, s, (int)bits, (int)group, w) == KVQ_TREE_PREFILL)
       return none();  // (its exponents are computed)
     const size_t need = d.tree_ws(b, hq, hk, l, dd, s, w);
     if (need == 0) return none();
@@ -681,7 +681,7 @@ PyObject* bind_draft(PyObject*, PyObject* const* a, Py_ssize_t n) {
   for (int i = 0; i < 11; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
   auto set = [&, i = 0](auto& fn) mutable { fn = (std::decay_t<decltype(fn)>)at[i++]; };
-  set(d.draft_tree), set(d.tree), set(d.tree_dense), set(d.tree_paged), set(d.tree_ws), set(d.tree_range);
+  set(d.draft_tree), set(d.tree), set(d.tree_dense), set(d.tree_paged), set(d.tree_ws), set(d.tree_kernel);
   set(d.rope_axes), set(d.axes_append), set(d.dequantize), set(d.paged_dequantize), set(d.keep_rows);
   return none();
 }

@@ -43,6 +43,7 @@ hipError_t launch_decode_dense(const kvq_rows* q, const kvq_rows* k, const kvq_r
                                const kvq_mask* mask = nullptr, const kvq_tree* tree = nullptr, bool tree_rows = false);
 
 size_t tree_rows_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
+float tree_rows_time(int B, int Hq, int Hkv, int L, int D, int S, int window, int bits);  // us, by a model
 size_t prefill_workspace_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window);
 hipError_t launch_prefill(const kvq_rows* q, const kvq_qtensor* k, const kvq_qtensor* v, const int32_t* seq_lens,
                           const kvq_rows* out, int B, int Hq, int Hkv, int L, int D, int S, int bits, int G, int dtype,

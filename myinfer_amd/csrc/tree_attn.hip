@@ -8,10 +8,13 @@ namespace kvq {
 
 struct TreePlan {
   int rowblocks, nunits, nsplit, fused;
+  float us;  // its time by the model
 };
 
-// Splits for about two workgroups a CU (one where the ring of an unquantized head_dim-128 cache fills a CU's LDS), each of
-// at least two tiles a wave.
+// The number of splits of least time by a rough model of a launch, in us: a wave's 32-key tile takes 2.1 with two workgroups
+// on its CU and 1.3 with one (half of it at 64 dims; the ring of an unquantized head_dim-128 cache leaves room for one), a
+// workgroup's start and its waves' merge 5, the splits' merge 1.5 by the last to finish, else a launch, its bytes and
+// the splits past the 32 that it loads at once. A wave gets at least two tiles.
 static TreePlan tree_plan(int B, int Hq, int Hkv, int L, int D, int S, int window, int bits) {
   TreePlan pl;
   const int nrows = (Hq / Hkv) * L;
@@ -19,9 +22,18 @@ static TreePlan tree_plan(int B, int Hq, int Hkv, int L, int D, int S, int windo
   pl.nunits = B * Hkv * pl.rowblocks;
   const int span = window > 0 ? std::min(S, window + L - 1 + kTile - 1) : S;
   const int tiles = (span + kTile - 1) / kTile;
-  const int target = bits == 16 && D == 128 ? 256 : 512;
-  const int most = std::max(1, tiles / (2 * kTW));
-  pl.nsplit = std::max(1, std::min({target / pl.nunits, most, kMaxSplit}));
+  const int per_cu = bits == 16 && D == 128 ? 1 : 2;
+  const int most = std::max(1, std::min(tiles / (2 * kTW), kMaxSplit));
+  pl.nsplit = 0;
+  for (int ns = 1; ns <= most; ns += ns < 16 ? 1 : ns / 8) {
+    const int64_t wgs = (int64_t)pl.nunits * ns, rounds = wgs / (256 * per_cu), rest = wgs % (256 * per_cu);
+    const float per = ((tiles + ns - 1) / ns + kTW - 1) / kTW * (D == 64 ? 0.5f : 1.0f);
+    const float one = per * 1.3f + 5.0f, two = per * (per_cu == 2 ? 2.1f : 1.3f) + 5.0f;
+    const bool fused = ns <= kFewSplits && pl.nunits <= kMaxCountedUnits;
+    const float merge = ns == 1 ? 0.0f : fused ? 1.5f : 3.5f + (float)wgs * (32 * D * 4) / 3e6f + (ns > 32 ? 0.06f * (ns - 32) : 0.0f);
+    const float t = rounds * two + (rest > 256 ? two : rest > 0 ? one : 0.0f) + merge;
+    if (pl.nsplit == 0 || t < pl.us) pl.nsplit = ns, pl.us = t;
+  }
   pl.fused = pl.nsplit <= kFewSplits && pl.nunits <= kMaxCountedUnits;
   return pl;
 }
@@ -38,6 +50,11 @@ static TreeLayout tree_layout(const TreePlan& pl, int D) {
   l.o = l.ml + up(rows * sizeof(float2));
   l.total = l.o + up(rows * D * sizeof(float));
   return l;
+}
+
+// (the model's time against 260 measured calls: 5.3 + 0.82 of it, within 16%)
+float tree_rows_time(int B, int Hq, int Hkv, int L, int D, int S, int window, int bits) {
+  return 5.3f + 0.82f * tree_plan(B, Hq, Hkv, L, D, S, window, bits).us;
 }
 
 size_t tree_rows_bytes(int B, int Hq, int Hkv, int L, int D, int S, int window) {

@@ -922,12 +922,12 @@ def _check_tree_call(tree: DraftTree, B: int, L: int, S: int, window: int, causa
 
 
 @functools.lru_cache(maxsize=256)
-def _tree_sizes(*sizes: int) -> Tuple[int, int]:
+def _tree_sizes(*sizes: int) -> Tuple[int, bool]:
     """(workspace bytes, whether a bf16 cache's range words are read) of a tree call, which follow from its sizes."""
-    B, Hq, Hkv, L, D, S, group_size, window = sizes
+    B, Hq, Hkv, L, D, S, bits, group_size, window = sizes
     lib = _lib.lib()
     return (lib.kvq_tree_workspace_size(B, Hq, Hkv, L, D, S, window),
-            lib.kvq_tree_reads_range(B, Hq, Hkv, L, D, S, group_size, window))
+            lib.kvq_tree_kernel(B, Hq, Hkv, L, D, S, bits, group_size, window) == _lib.TREE_PREFILL)
 
 
 def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq_lens, group_size, bits, causal, kernel,
@@ -937,7 +937,7 @@ def _prepare_tree(queries, keys, values, scale, tree, out, *, dense, window, seq
     dev = queries.device
     Hkv, S = keys.shape[1:3] if dense else keys[0].shape[1:3]
     _check_tree_call(tree, B, L, S, window, causal, kernel, dev)
-    nbytes, ranges = _tree_sizes(B, Hq, Hkv, L, D, S, 64 if dense else group_size, int(window))
+    nbytes, ranges = _tree_sizes(B, Hq, Hkv, L, D, S, 16 if dense else int(bits), 64 if dense else int(group_size), int(window))
     if nbytes == 0:
         raise NotImplementedError(f"tree attention does not support B={B} Hq={Hq} Hkv={Hkv} L={L} D={D} S={S}")
     stream = _lib.stream_ptr(dev)
@@ -1391,7 +1391,7 @@ def paged_attention(queries: torch.Tensor, k_pool: Triple, v_pool: Triple, block
     if tree is not None:
         block_tables = _whole_table(block_tables, B, dev)
         _check_tree_call(tree, B, L, S, window, causal, kernel, dev)
-        nbytes, _ = _tree_sizes(B, Hq, Hkv, L, D, S, int(group_size), int(window))
+        nbytes, _ = _tree_sizes(B, Hq, Hkv, L, D, S, int(bits), int(group_size), int(window))
         if nbytes == 0:
             raise NotImplementedError(f"tree attention does not support B={B} Hq={Hq} Hkv={Hkv} L={L} D={D} S={S}")
         stream = _lib.stream_ptr(dev)

@@ -17,39 +17,34 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
-def on_rows_kernel(B, Hq, Hkv, D, G, L, S, window=0):
-    """The rule by sizes: passes of 16 G / D rows past the third, and blocks of 32 rows past the fourth."""
-    rows, keys = Hq // Hkv * L, min(S, window + L) if window else S
-    work = B * Hkv * keys * D
-    passes, blocks = -(-rows // (16 * G // D)), -(-rows // 32)
-    return rows > 8 and (passes - 3) * work >= 1 << 25 and (blocks - 4) * work <= 1 << 25
+def on_rows_kernel(B, Hq, Hkv, D, G, L, S, window=0, bits=8):
+    return _lib.lib().kvq_tree_kernel(B, Hq, Hkv, L, D, S, bits, G, window) == _lib.TREE_ROWS
 
 
 CASES = [
     # (B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window)
     (1, 64, 4, 128, 64, 8, torch.float16, 21, 2049, "random", 0),    # 336 rows, 16 splits
     (2, 64, 8, 128, 64, 8, torch.bfloat16, 33, 577, "gaps", 0),      # few splits, merged by the last
-    (8, 64, 8, 128, 64, 4, torch.float16, 64, 130, "random", 0),     # one split
+    (8, 64, 8, 128, 64, 4, torch.float16, 30, 130, "random", 0),     # one split
     (2, 32, 4, 128, 64, 4, torch.bfloat16, 30, 1409, "gaps", 0),
     (1, 64, 8, 128, 32, 8, torch.float16, 17, 1100, "random", 0),    # four groups a row
     (2, 64, 4, 128, 32, 4, torch.bfloat16, 13, 1023, "gaps", 0),
-    (1, 32, 4, 128, 128, 8, torch.float16, 64, 2305, "star", 0),     # one group a row
-    (1, 32, 4, 128, 128, 4, torch.bfloat16, 59, 2500, "random", 0),
+    (1, 32, 4, 128, 128, 8, torch.float16, 64, 3500, "star", 0),     # one group a row
+    (1, 32, 4, 128, 128, 4, torch.bfloat16, 59, 3500, "random", 0),
     (4, 64, 8, 64, 64, 8, torch.float16, 33, 1201, "chain", 0),
     (2, 64, 8, 64, 64, 4, torch.bfloat16, 40, 2100, "gaps", 0),
     (2, 64, 8, 64, 32, 8, torch.bfloat16, 24, 1601, "random", 0),
     (4, 64, 8, 64, 32, 4, torch.float16, 29, 900, "gaps", 0),
     (4, 64, 8, 128, 64, 8, torch.float16, 64, 600, "random", 80),    # windows: the first keys hidden from all
     (4, 64, 8, 128, 64, 4, torch.bfloat16, 40, 700, "gaps", 200),
-    (8, 64, 8, 128, 64, 8, torch.float16, 70, 70, "random", 0),      # no prefix
+    (4, 64, 8, 128, 64, 8, torch.float16, 33, 33, "random", 0),      # no prefix
 ]
 
 
 @pytest.mark.parametrize("B,Hq,Hkv,D,G,bits,dtype,L,S,kind,window", CASES)
 def test_quantized(B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window):
     print(f"tree rows B={B} Hq={Hq} Hkv={Hkv} D={D} G={G} bits={bits} {dtype} L={L} S={S} {kind} window={window}", flush=True)
-    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window)
-    assert _lib.lib().kvq_tree_reads_range(B, Hq, Hkv, L, D, S, G, window) == 0  # (which only the prefill kernel does)
+    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window, bits)
     kt, vt = make_cache(B, Hkv, S, D, bits, dtype, 340 + L, group=G)
     q = seeded_normal((B, Hq, L, D), 341 + S, dtype, DEV)
     parents = make_parents(kind, B, L, 342 + D)
@@ -65,14 +60,14 @@ def test_quantized(B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window):
 @pytest.mark.parametrize("B,Hq,Hkv,D,dtype,L,S,kind,window", [
     (1, 64, 4, 128, torch.float16, 20, 2047, "random", 0),
     (2, 64, 8, 128, torch.bfloat16, 40, 650, "gaps", 0),
-    (4, 64, 16, 128, torch.bfloat16, 64, 150, "random", 0),
-    (4, 64, 8, 64, torch.float16, 40, 1000, "gaps", 0),
-    (2, 64, 8, 64, torch.bfloat16, 40, 2050, "random", 0),
-    (4, 64, 8, 128, torch.float16, 40, 700, "random", 200),
+    (4, 64, 16, 128, torch.bfloat16, 30, 150, "random", 0),
+    (4, 64, 8, 64, torch.float16, 40, 2000, "gaps", 0),
+    (2, 64, 8, 64, torch.bfloat16, 40, 4100, "random", 0),
+    (4, 64, 8, 128, torch.float16, 30, 700, "random", 200),
 ])
 def test_unquantized(B, Hq, Hkv, D, dtype, L, S, kind, window):
     print(f"tree rows unquantized B={B} Hq={Hq} Hkv={Hkv} D={D} {dtype} L={L} S={S} {kind} window={window}", flush=True)
-    assert on_rows_kernel(B, Hq, Hkv, D, 64, L, S, window)
+    assert on_rows_kernel(B, Hq, Hkv, D, 64, L, S, window, 16)
     k, v = (seeded_normal((B, Hkv, S, D), 350 + i, dtype, DEV) for i in range(2))
     q = seeded_normal((B, Hq, L, D), 352, dtype, DEV)
     parents = make_parents(kind, B, L, 353)
@@ -91,12 +86,12 @@ def test_unquantized(B, Hq, Hkv, D, dtype, L, S, kind, window):
     (2, 64, 8, 64, 32, 8, torch.bfloat16, 80, 2111, "random", 0),
     (2, 64, 8, 128, 64, 8, torch.float16, 100, 1500, "random", 1300),
     (2, 64, 8, 128, 64, 16, torch.bfloat16, 64, 1500, "gaps", 0),
-    (4, 64, 8, 64, 64, 16, torch.float16, 64, 1450, "random", 0),
+    (4, 64, 8, 64, 64, 16, torch.float16, 100, 1450, "random", 0),
 ])
 def test_past_the_rows_kernel(B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window):
     """Sizes beyond the line to the prefill kernel."""
     print(f"tree prefill B={B} Hq={Hq} Hkv={Hkv} D={D} G={G} bits={bits} {dtype} L={L} S={S} {kind} window={window}", flush=True)
-    assert not on_rows_kernel(B, Hq, Hkv, D, G, L, S, window)
+    assert _lib.lib().kvq_tree_kernel(B, Hq, Hkv, L, D, S, bits, G, window) == _lib.TREE_PREFILL
     q = seeded_normal((B, Hq, L, D), 331 + S, dtype, DEV)
     parents = make_parents(kind, B, L, 332 + D)
     scale = 1.0 / math.sqrt(D)
@@ -130,7 +125,7 @@ def test_paged_unequal_lengths(Hq, Hkv, D, G, bits, dtype, L, window):
     print(f"tree rows paged Hq={Hq} Hkv={Hkv} D={D} G={G} bits={bits} {dtype} L={L} window={window}", flush=True)
     lens = [L, 640, 641, 1999]
     B, S = len(lens), max(lens)
-    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window) == (L < 70)
+    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window, bits) == (L < 70)
     _, tables, kp, vp, kc, vc = build(B, Hkv, lens, D, bits, dtype, 360, group=G)
     if dtype == torch.bfloat16:
         for tr in (kp, vp):
@@ -222,8 +217,8 @@ def test_bf16_ranges_by_tile(G, bits, D):
     """K and V rows of a bf16 cache whose magnitudes grow and shrink by powers of two from tile to tile, up to 2^40 (K
     2^20): every power of two is exact. With V's, queries of zero weigh all keys alike; with K's, queries of 2^-19 keep the
     scores of the usual size, so that the operands' rounding moves them as little as in the other tests."""
-    Hq, Hkv, L, S, B = 64, 8, 30, 3000 if 16 * G // D > 8 else 1500, 2
-    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S)
+    Hq, Hkv, L, S, B = 64, 8, 30, 2000 if 16 * G // D > 8 else 1500, 2
+    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, 0, bits)
     kt, vt = make_cache(B, Hkv, S, D, bits, torch.bfloat16, 420, group=G)
     p2 = torch.ones(S, dtype=torch.float32)
     for at, n, e in [(64, 40, 20), (333, 5, 40), (700, 1, 17), (1201, 64, 33)]:

@@ -123,9 +123,12 @@ def test_tree_workspace_covers_both_kernels():
             assert n >= lib.kvq_decode_workspace_size(2, 32, 8, L, D, 5000, 0) > 0
     assert lib.kvq_tree_workspace_size(2, 30, 8, 4, 128, 5000, 0) == 0
     assert lib.kvq_tree_workspace_size(2, 32, 8, 0, 128, 5000, 0) == 0
-    # few rows stay on the decode kernel, which reads no range words
-    assert lib.kvq_tree_reads_range(1, 8, 8, 8, 128, 5000, 64, 0) == 0
-    assert lib.kvq_tree_reads_range(1, 64, 8, 64, 128, 32768, 64, 0) == 1
+    # few rows stay on the decode kernel, tens and hundreds take kernels of their own
+    assert lib.kvq_tree_kernel(1, 8, 8, 8, 128, 5000, 8, 64, 0) == _lib.TREE_DECODE
+    assert lib.kvq_tree_kernel(1, 64, 8, 8, 128, 32768, 8, 64, 0) == _lib.TREE_ROWS
+    assert lib.kvq_tree_kernel(1, 64, 8, 64, 128, 32768, 8, 64, 0) == _lib.TREE_PREFILL
+    assert lib.kvq_tree_kernel(1, 64, 8, 64, 256, 32768, 16, 64, 0) == _lib.TREE_DECODE  # (one kernel at 256 dims unquantized)
+    assert lib.kvq_tree_kernel(1, 30, 8, 64, 128, 32768, 8, 64, 0) == _lib.TREE_DECODE  # (no such call)
 
 
 def test_draft_tree_refuses():
