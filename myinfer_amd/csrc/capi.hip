@@ -749,10 +749,11 @@ static int check_tree(const kvq_tree* t, int L, float scale, int window) {
 }
 
 // The kernel of a tree call by its sizes: the one whose time is estimated the lowest. rows: a KV head's query rows.
-//   decode: a launch and 25 us (64 dims 18, unquantized 12.5) for a million keys of a pass of 16 G / D rows, and 2.5 for
-//           512 workgroups of it (unquantized 64 dims none);
-//   rows:   its plan's model (tree_attn.hip);
-//   prefill: a launch or two and 85 us (130) for a million keys of a block of 256 rows.
+//   decode: a launch, 25 us (64 dims 18, unquantized 12.5; 96 dims 30; 256 dims 35) for a million keys of a pass of 16 G / D
+//           rows (D the kernel's width), and 2.5 for 512 workgroups of it (unquantized 64 dims none);
+//   rows:   its plan's model (tree_attn.hip), 64 and 128 dims;
+//   prefill: a launch or two and 130 us (64 dims 85, 96 dims 100) for a million keys of a block of 256 rows; 256 dims:
+//           145 of 128 rows.
 // Over 260 random calls the choice came to 1.6% more than the best of the three on average (a choice by rows and keys
 // alone 5%), 41% at most. us, decode / rows / prefill (128 dims, groups of 64, 8 bits, 8 KV heads unless said):
 //   20 rows,  4106 keys   11.5 /  13.8 /  22    32 rows, 8 sequences of 4096, 4 bits  32.5 / 26.2 / 53.0
@@ -762,24 +763,22 @@ static int check_tree(const kvq_tree* t, int L, float scale, int window) {
 //  256 rows,  2048 keys   20.6 /  20.7 /  24   256 rows, 32768 keys                    215 / 79.9 / 59.6
 //  124 rows of 64 unquantized dims, 4 sequences of 2047: 11.0 / 11.9 / 22; 44 rows of 64 dims, 64 units of 19345: 105 / 60 / 111
 //  928 unquantized rows, 32 units of 265: 90 / 39.5 / 19.3
-// head_dim 96 has no rows kernel, head_dim 256 neither: its prefill kernel's lines are kernels._auto_kernel's.
+// At 96 and 256 dims, of two, 1.2% and 1.9% above the better over 70 random calls each (choices by rows and passes 16% and
+// 5%, 334% and 104% at most).
 enum class TreeKernel { kDecode, kRows, kPrefill };
 static TreeKernel tree_kernel_of(int B, int Hq, int Hkv, int L, int D, int S, int bits, int group_size, int window) {
   const bool dense = bits == 16;
   const int64_t rows = (int64_t)(Hq / Hkv) * L, units = (int64_t)B * Hkv;
   const int64_t keys = window > 0 ? std::min((int64_t)S, (int64_t)window + L) : S;
-  if (D == 96 && !dense) return rows > 64 ? TreeKernel::kPrefill : TreeKernel::kDecode;
-  if ((D != 64 && D != 128 && D != 256) || (D == 256 && dense)) return TreeKernel::kDecode;
-  if (rows <= 8) return TreeKernel::kDecode;
-  const int64_t per = 16 * group_size / D, passes = (rows + per - 1) / per;
-  if (D == 256) {
-    const bool few = rows < 128 && units * passes <= 512 && (passes - 3) * units * keys <= 5 << 15;
-    return few ? TreeKernel::kDecode : TreeKernel::kPrefill;
-  }
+  if ((D != 64 && D != 96 && D != 128 && D != 256) || (dense && D != 64 && D != 128) || rows <= 8) return TreeKernel::kDecode;
+  const int64_t per = std::max(16 * (int64_t)group_size / (D == 96 ? 128 : D), (int64_t)1), passes = (rows + per - 1) / per;
+  const int64_t block = D == 256 ? 128 : 256, blocks = (rows + block - 1) / block;
   const float work = (float)(units * keys) * 1e-6f;
-  const float pass = D != 64 ? 25.0f : dense ? 12.5f : 18.0f, group = D == 64 && dense ? 0.0f : 2.5f / 512;
-  const float decode = 7.5f + pass * work * passes + group * (float)(units * passes);
-  const float prefill = 14.5f + (D == 64 ? 85.0f : 130.0f) * work * ((rows + 255) / 256);
+  const float pass_us = D == 256 ? 35.0f : D == 128 ? 25.0f : D == 96 ? 30.0f : dense ? 12.5f : 18.0f;
+  const float block_us = D == 256 ? 145.0f : D == 128 ? 130.0f : D == 96 ? 100.0f : 85.0f;
+  const float decode = 7.5f + pass_us * work * passes + (D == 64 && dense ? 0.0f : 2.5f / 512) * (float)(units * passes);
+  const float prefill = (D == 256 ? 16.0f : 14.5f) + block_us * work * blocks;
+  if (D == 96 || D == 256) return decode <= prefill ? TreeKernel::kDecode : TreeKernel::kPrefill;
   const float mine = kvq::tree_rows_time(B, Hq, Hkv, L, D, S, window, bits);
   return decode <= mine && decode <= prefill ? TreeKernel::kDecode : mine <= prefill ? TreeKernel::kRows : TreeKernel::kPrefill;
 }

@@ -83,17 +83,17 @@ QUANT = [
     (1, 16, 8, 128, 64, 8, torch.float16, 10, 4106, "random", 0),
     (2, 8, 2, 128, 64, 8, torch.bfloat16, 33, 33, "gaps", 0),       # no prefix
     (2, 32, 4, 128, 64, 4, torch.float16, 16, 1000, "random", 0),
-    (1, 64, 8, 128, 64, 8, torch.bfloat16, 64, 2111, "gaps", 0),    # rows kernel
+    (1, 64, 8, 128, 64, 8, torch.bfloat16, 64, 2111, "gaps", 0),
     (1, 8, 1, 128, 128, 4, torch.bfloat16, 130, 777, "random", 0),
     (1, 32, 4, 128, 32, 8, torch.float16, 31, 513, "random", 0),
     (1, 16, 2, 64, 64, 8, torch.bfloat16, 65, 900, "random", 0),
     (2, 8, 8, 64, 32, 4, torch.float16, 7, 95, "gaps", 0),
     (1, 32, 2, 64, 64, 4, torch.float16, 40, 6000, "random", 0),
     (1, 8, 4, 256, 64, 8, torch.float16, 9, 700, "random", 0),
-    (1, 16, 2, 256, 128, 4, torch.bfloat16, 50, 1300, "gaps", 0),   # head_dim-256 kernel
+    (1, 16, 2, 256, 128, 4, torch.bfloat16, 50, 1300, "gaps", 0),
     (1, 8, 2, 256, 64, 8, torch.bfloat16, 100, 260, "random", 0),
-    (1, 8, 8, 96, 32, 8, torch.float16, 12, 333, "random", 0),      # narrow rows, decode kernel
-    (1, 32, 4, 96, 32, 4, torch.float16, 20, 901, "gaps", 0),       # ... prefill kernel
+    (1, 8, 8, 96, 32, 8, torch.float16, 12, 333, "random", 0),      # narrow rows
+    (1, 32, 4, 96, 32, 4, torch.float16, 20, 901, "gaps", 0),
     (1, 4, 4, 32, 32, 8, torch.bfloat16, 5, 77, "random", 0),
     (1, 8, 4, 192, 64, 4, torch.float16, 6, 300, "random", 0),
     (1, 16, 8, 128, 64, 8, torch.float16, 10, 2000, "random", 64),  # windows

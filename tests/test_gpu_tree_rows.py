@@ -87,9 +87,14 @@ def test_unquantized(B, Hq, Hkv, D, dtype, L, S, kind, window):
     (2, 64, 8, 128, 64, 8, torch.float16, 100, 1500, "random", 1300),
     (2, 64, 8, 128, 64, 16, torch.bfloat16, 64, 1500, "gaps", 0),
     (4, 64, 8, 64, 64, 16, torch.float16, 100, 1450, "random", 0),
+    (1, 32, 4, 256, 64, 8, torch.float16, 30, 2100, "gaps", 0),      # the head_dim-256 kernel
+    (2, 32, 4, 256, 128, 4, torch.bfloat16, 33, 1500, "random", 0),
+    (2, 32, 4, 256, 64, 8, torch.bfloat16, 40, 1501, "gaps", 900),
+    (1, 64, 8, 96, 32, 8, torch.bfloat16, 20, 1900, "gaps", 0),      # the 96-wide one
+    (2, 32, 4, 96, 32, 4, torch.float16, 45, 1500, "random", 1100),
 ])
 def test_past_the_rows_kernel(B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window):
-    """Sizes beyond the line to the prefill kernel."""
+    """Sizes whose estimate is lowest for the prefill kernels."""
     print(f"tree prefill B={B} Hq={Hq} Hkv={Hkv} D={D} G={G} bits={bits} {dtype} L={L} S={S} {kind} window={window}", flush=True)
     assert _lib.lib().kvq_tree_kernel(B, Hq, Hkv, L, D, S, bits, G, window) == _lib.TREE_PREFILL
     q = seeded_normal((B, Hq, L, D), 331 + S, dtype, DEV)
@@ -116,6 +121,8 @@ def test_past_the_rows_kernel(B, Hq, Hkv, D, G, bits, dtype, L, S, kind, window)
     (64, 8, 128, 128, 8, torch.float16, 37, 500),
     (64, 8, 128, 64, 8, torch.bfloat16, 70, 0),    # the prefill kernel
     (64, 8, 64, 64, 4, torch.float16, 111, 0),
+    (32, 4, 256, 128, 8, torch.bfloat16, 33, 0),
+    (32, 4, 96, 32, 4, torch.bfloat16, 40, 0),
 ])
 def test_paged_unequal_lengths(Hq, Hkv, D, G, bits, dtype, L, window):
     """Pages in a shuffled order whose unused rows hold NaN scales; one sequence is its tree alone, one tree ends on
@@ -125,7 +132,8 @@ def test_paged_unequal_lengths(Hq, Hkv, D, G, bits, dtype, L, window):
     print(f"tree rows paged Hq={Hq} Hkv={Hkv} D={D} G={G} bits={bits} {dtype} L={L} window={window}", flush=True)
     lens = [L, 640, 641, 1999]
     B, S = len(lens), max(lens)
-    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window, bits) == (L < 70)
+    assert on_rows_kernel(B, Hq, Hkv, D, G, L, S, window, bits) == (L < 70 and D in (64, 128))
+    assert _lib.lib().kvq_tree_kernel(B, Hq, Hkv, L, D, S, bits, G, window) != _lib.TREE_DECODE
     _, tables, kp, vp, kc, vc = build(B, Hkv, lens, D, bits, dtype, 360, group=G)
     if dtype == torch.bfloat16:
         for tr in (kp, vp):

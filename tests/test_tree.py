@@ -129,6 +129,11 @@ def test_tree_workspace_covers_both_kernels():
     assert lib.kvq_tree_kernel(1, 64, 8, 64, 128, 32768, 8, 64, 0) == _lib.TREE_PREFILL
     assert lib.kvq_tree_kernel(1, 64, 8, 64, 256, 32768, 16, 64, 0) == _lib.TREE_DECODE  # (one kernel at 256 dims unquantized)
     assert lib.kvq_tree_kernel(1, 30, 8, 64, 128, 32768, 8, 64, 0) == _lib.TREE_DECODE  # (no such call)
+    for group in (0, 1, 8, -64):  # no such groups: any answer, but an answer
+        assert lib.kvq_tree_kernel(1, 64, 8, 64, 256, 32768, 8, group, 0) in (0, 1, 2)
+    for D in (96, 256):  # two kernels
+        assert lib.kvq_tree_kernel(1, 64, 8, 64, D, 4096, 8, 64 if D > 96 else 32, 0) == _lib.TREE_PREFILL
+        assert lib.kvq_tree_kernel(1, 64, 8, 2, D, 300, 8, 64 if D > 96 else 32, 0) == _lib.TREE_DECODE
 
 
 def test_draft_tree_refuses():
