@@ -141,7 +141,8 @@ __device__ __forceinline__ void quantize_chunk(const float (&x)[EPT], bool activ
   // half-integer lies within one ulp. A thread with any quotient within 2 ulp (|q1| 2^-22) of a
   // half-integer, or of magnitude 2^21 or more, or not finite, divides all its elements exactly:
   // the codes stay bit-identical and the division is the rare path.
-  auto& packed = z.packed;
+  constexpr int W = Quantized<BITS, EPT>::W;
+  uint32_t packed[W];
   float low = 0.0f;  // 4 bits: the code before, the low nibble of its byte
   auto put = [&](int i, float c) {
     if constexpr (BITS == 8) {
@@ -176,6 +177,8 @@ __device__ __forceinline__ void quantize_chunk(const float (&x)[EPT], bool activ
 #pragma unroll
     for (int i = 0; i < EPT; ++i) put(i, rintf((x[i] - bias) / s));
   }
+#pragma unroll
+  for (int w = 0; w < W; ++w) z.packed[w] = packed[w];
   z.s = s;
   z.bias = bias;
 }
