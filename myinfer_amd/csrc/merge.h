@@ -129,8 +129,9 @@ __global__ __launch_bounds__(256) void combine_kernel(MergeParams p, int nrows, 
   *(u2*)dst = w;
 }
 
-template <typename T, int D>
-// dv: dims of an output row (D unless the decode kernel ran narrower rows at width D)
+// dv: dims of an output row (D unless the decode kernel ran narrower rows at width D); ONLY: the R of every call there is,
+// or 0 for the kernels whose R follows from their groups
+template <typename T, int D, int ONLY = 0>
 inline hipError_t launch_combine(const MergeParams& m, int B, hipStream_t stream, int dv = D) {
   const int nrows = B * m.Hq * m.L;
   constexpr int rpb = 256 / D;  // rows per 256-thread workgroup
@@ -142,6 +143,11 @@ inline hipError_t launch_combine(const MergeParams& m, int B, hipStream_t stream
   mm.d_rep = make_div31((uint32_t)m.rep);
   // R (rows per unit: 16 / scale groups per row for decode, 32 for the tree rows kernel, 128 for the head_dim-256
   // kernel) fixes the kernel's split strides
+  if constexpr (ONLY != 0) {
+    if (m.R != ONLY || dv != D) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((combine_kernel<T, D, ONLY>), grid, dim3(256), 0, stream, mm, nrows, dv);
+    return hipGetLastError();
+  }
   if (dv != D) {
     switch (m.R) {
       case 4: hipLaunchKernelGGL((combine_kernel<T, D, 4, true>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
@@ -156,12 +162,6 @@ inline hipError_t launch_combine(const MergeParams& m, int B, hipStream_t stream
     case 4: hipLaunchKernelGGL((combine_kernel<T, D, 4>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 8: hipLaunchKernelGGL((combine_kernel<T, D, 8>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     case 16: hipLaunchKernelGGL((combine_kernel<T, D, 16>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
-    case 32:
-      if constexpr (D <= 128) {
-        hipLaunchKernelGGL((combine_kernel<T, D, 32>), grid, dim3(256), 0, stream, mm, nrows, dv);
-        break;
-      }
-      return hipErrorInvalidValue;
     case 128: hipLaunchKernelGGL((combine_kernel<T, D, 128>), grid, dim3(256), 0, stream, mm, nrows, dv); break;
     default: return hipErrorInvalidValue;
   }

@@ -68,7 +68,7 @@ static hipError_t launch_t(const DecParams& p, int B, hipStream_t stream) {
   hipLaunchKernelGGL((tree_attn_kernel<T, D, BITS, G, PAGED>), dim3(p.nunits * p.nsplit), dim3(kTW * 64), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.nsplit == 1 || p.fused) return e;
-  return launch_combine<T, D>(merge_params(p, 32), B, stream);
+  return launch_combine<T, D, 32>(merge_params(p, 32), B, stream);
 }
 
 hipError_t launch_tree_rows(DecParams p, int B, int dtype, int D, int bits, int G, bool paged, void* workspace, hipStream_t stream) {
