@@ -240,7 +240,9 @@ PyObject* views(PyObject*, PyObject* const* a, Py_ssize_t n) {
           Py_DECREF(both);
           return none();
         }
-        PyTuple_SET_ITEM(tr, j, THPVariable_Wrap(x[j]->narrow(-2, 0, rows)));
+        c10::SmallVector<int64_t, 8> size(x[j]->sizes().begin(), x[j]->sizes().end());
+        size[size.size() - 2] = rows;
+        PyTuple_SET_ITEM(tr, j, THPVariable_Wrap(x[j]->as_strided(size, x[j]->strides(), x[j]->storage_offset())));
       }
     }
     return both;
