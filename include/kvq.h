@@ -157,7 +157,8 @@ typedef struct kvq_axes {
   int64_t pos_stride_a, pos_stride_b, pos_stride_l;
 } kvq_axes;
 
-/* In-place rotation of rows [0, L) of x (T[B][H][L][D]) by `rope`. */
+/* In-place rotation of rows [0, L) of x (T[B][H][L][D]) by `rope`. Rows that share their memory (a stride of 0) are
+ * refused, here and where kvq_rope_axes_append rotates q and kvq_dequantize writes. */
 int kvq_rope_axes(const kvq_rows* x, const kvq_axes* rope, int B, int H, int L, int D, int dtype, void* stream);
 
 /*
@@ -447,6 +448,7 @@ typedef struct kvq_row_array {
  * block_table NULL: contiguous arrays, rows [start, start + n) of each (starts must be NULL). Else paged pools,
  * start of sequence b starts[b] (device int32 [B], or NULL: `start`); a row whose page is outside the table, or whose
  * entry is outside [0, num_pages), is neither read nor written. The pages moved into must belong to one sequence.
+ * The arrays must not overlap: one named twice, or broadcast (a stride of 0), is refused.
  * M <= n; B <= 65535.
  */
 int kvq_keep_rows(const kvq_row_array* arrays, int n_arrays, int num_pages, const int32_t* block_table,

@@ -443,7 +443,8 @@ def keep_rows(cache: List, start: int, rows: torch.Tensor) -> int:
     """After the rows from `start` on were drafted and verified: keep those that `rows` names (int32 [B, M] or [M] on
     the GPU, indices from `start` in ascending order, the accepted path of a tree), move them up to rows start ..
     start + M - 1 in every layer's cache, and drop the rest, as ``trim_prompt_cache`` drops a rejected tail. One
-    launch for up to 32 layers. The caches are KVCache or QuantizedKVCache at one offset; returns the new one."""
+    launch for up to 32 layers. The caches are KVCache or QuantizedKVCache at one offset, none of them named twice;
+    returns the new offset."""
     if not cache:
         raise ValueError("no caches")
     if not torch.is_tensor(rows):

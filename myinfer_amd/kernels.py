@@ -208,7 +208,7 @@ _axes_desc = functools.lru_cache(maxsize=64)(RopeAxes.params)
 
 def rope_axes(x: torch.Tensor, r: RopeAxes, positions: torch.Tensor) -> torch.Tensor:
     """Rotate x [B, H, L, D] (float16/bfloat16, CUDA) in place, row l of sequence b at positions[:, b, l], and return
-    it. positions: int32 [axes, B, L] or [axes, L]."""
+    it. positions: int32 [axes, B, L] or [axes, L]. A broadcast x, whose rows share their memory, is refused."""
     host, stream = _native(x)
     if host is not None:
         desc = _axes_desc(r)
@@ -1306,8 +1306,8 @@ def keep_rows(tensors: Sequence[torch.Tensor], rows: torch.Tensor, start: int, n
     """Move the accepted rows of drafted ones up, in place: in every array [B, H, cap, W] of `tensors` (codes, scales,
     biases, or unquantized rows; any mix of layers), row start + i of sequence b becomes what row start + rows[b, i] held,
     for the M entries of rows (int32 [B, M] or [M], on the GPU; indices among the n rows from `start`). An entry outside
-    [i, n) leaves its row as it is, so an ascending list padded with -1 keeps fewer rows for some sequences. One launch for
-    up to 192 arrays."""
+    [i, n) leaves its row as it is, so an ascending list padded with -1 keeps fewer rows for some sequences. An array named
+    twice, or broadcast, is refused. One launch for up to 192 arrays."""
     tensors = list(tensors)
     if move_rows(tensors, rows, start, n):
         return

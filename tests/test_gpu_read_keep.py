@@ -173,6 +173,30 @@ def test_keep_rows_of_many_layers_and_shared_list():
         assert torch.equal(bits_of(t), reference_move(old, start, [rows] * B, n))
 
 
+def test_shared_memory_refused():
+    """The same cache twice, and tensors broadcast along an axis, before anything moves; an axis of one row may have any stride."""
+    c = QuantizedKVCache(64, 8)
+    c.update_and_fetch(*(seeded_normal((2, 2, 20, 128), 70 + j, torch.float16, DEV) for j in range(2)))
+    before = [bits_of(t).clone() for t in (*c.keys, *c.values)]
+    rows = torch.tensor([1, 3], dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="twice"):
+        keep_rows([c, c], 10, rows)
+    assert c.offset == 20 and all(torch.equal(bits_of(t), b) for t, b in zip((*c.keys, *c.values), before))
+    one = seeded_normal((1, 1, 3, 128), 72, torch.float16, DEV)
+    for shape in ((2, 1, 3, 128), (1, 2, 3, 128)):
+        with pytest.raises(ValueError, match="broadcast"):
+            kernels.keep_rows([one.expand(shape)], rows[:1], 0, 3)
+        with pytest.raises(ValueError, match="share"):
+            kernels.rope_axes(one.expand(shape), kernels.RopeAxes(128), torch.zeros(1, 3, dtype=torch.int32, device=DEV))
+        with pytest.raises(ValueError, match="share"):
+            k = tuple(x[: shape[0], : shape[1], :3] for x in c.keys)
+            kernels.dequantize_rows(k, k, group_size=64, bits=8, out=(one.expand(shape), one.expand(shape)))
+    pos = torch.arange(3, dtype=torch.int32, device=DEV).view(1, 3)
+    strange = one.clone().as_strided((1, 1, 3, 128), (0, 0, 128, 1))
+    assert torch.equal(kernels.rope_axes(strange, kernels.RopeAxes(128), pos),
+                       kernels.rope_axes(one.clone(), kernels.RopeAxes(128), pos))
+
+
 def test_nothing_kept():
     c = QuantizedKVCache(64, 8)
     c.update_and_fetch(*(seeded_normal((1, 2, 20, 128), 50 + j, torch.float16, DEV) for j in range(2)))

@@ -186,6 +186,46 @@ def test_keep_rows_refuses():
     assert call(M=0) == _lib.OK and call(n_arrays=0) == _lib.OK and call(H=0) == _lib.OK
 
 
+def test_refuses_rows_that_share_their_memory():
+    # what is written in place, or out, has an address of its own for every row: of a broadcast tensor, or an array named
+    # twice, the result would depend on the order of the workgroups
+    lib = _lib.lib()
+    pos = 1 << 22
+
+    def rows(**kw):
+        r = _fake_rows()
+        for name, x in kw.items():
+            setattr(r, name, x)
+        return r
+
+    axes = kernels.RopeAxes(128).params()
+    axes.positions = pos
+    for name in ("stride_b", "stride_h", "stride_l"):
+        x = rows(**{name: 0})
+        _expect(lib.kvq_rope_axes(byref(x), byref(axes), 3, 4, 5, 128, 0, None), _lib.ERR_INVALID, "x")
+        _expect(lib.kvq_rope_axes_append(byref(rows()), byref(_fake_q()), None, None, byref(x), 4, byref(axes), 0, None, 0, None,
+                                         0, 3, 4, 5, 128, 8, 64, 0, None), _lib.ERR_INVALID, "queries")
+        _expect(lib.kvq_dequantize(byref(_fake_q()), byref(rows()), byref(_fake_q()), byref(x), 0, 3, 4, 5, 128, 8, 64, 0, None),
+                _lib.ERR_INVALID, "v_dst")
+        _expect(lib.kvq_paged_dequantize(byref(_pool()), byref(x), None, None, 4, 1 << 20, 2, 1 << 21, 3, 4, 5, 128, 8, 64, 0,
+                                         None), _lib.ERR_INVALID, "k_dst")
+
+    def keep(n, data, table=None, B=2, H=2, M=4, **kw):
+        a = dict(stride_b=4096, stride_h=1024, stride_l=128, row_bytes=128)
+        a.update(kw)
+        arr = (_lib.RowArray * n)(*(_lib.RowArray(data(i), *a.values()) for i in range(n)))
+        return lib.kvq_keep_rows(arr, n, 4 if table else 0, table, 4 if table else 0, 1 << 22, 4, None, 0, 8, M, B, H, None)
+
+    for n in (2, 6, 192, 200, 3000):  # the twin of the first array comes last
+        for table in (None, 1 << 23):
+            _expect(keep(n, lambda i: (1 << 24) + (i % (n - 1)) * 8192, table), _lib.ERR_INVALID, "twice")
+    _expect(keep(1, lambda i: 1 << 24, stride_b=0), _lib.ERR_INVALID, "broadcast")
+    _expect(keep(1, lambda i: 1 << 24, stride_h=0), _lib.ERR_INVALID, "broadcast")
+    _expect(keep(1, lambda i: 1 << 24, 1 << 23, stride_b=0, B=1), _lib.ERR_INVALID, "broadcast")  # (all pages one)
+    # arrays of their own are nothing to refuse
+    assert keep(3000, lambda i: (1 << 24) + i * 8192, M=0) == _lib.OK
+
+
 def test_python_refusals_on_the_host():
     x = torch.zeros(1, 2, 3, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="GPU"):
